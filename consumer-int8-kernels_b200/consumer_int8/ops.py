@@ -29,6 +29,18 @@ into caller-allocated outputs, returns ``None`` and can be captured in a CUDA gr
   peer_rendezvous(signal_ptrs CPU INT64[G], state INT64[2], rank)
       that rendezvous as a one-thread kernel of its own, to follow fused_channel_mm_gather
 
+The attention side of the layer, over a key/value cache held in 4 bits (UINT8 [pages, 2, kv_heads, kv4_block_bytes(page,
+dim)]: rows of 4-bit codes and a BF16 scale and zero point for each token and head; heads tensors are BF16 [tokens, heads,
+dim], dim 64, 128 or 256, and may be slices of one projection's output):
+
+  qk_norm_rope(q, k, q_weight?, k_weight?, cos_sin?, positions?, axis_of?, q_out, k_out, eps, weight_offset, adjacent)
+      RMS norm of every query and key head and the rotation to its position (one to four position axes), one launch
+  kv4_append(q?, k, v, cos_sin?, positions?, axis_of?, slots INT64[T], q_out?, cache, adjacent)
+      keys rotated on the way, keys and values encoded into the cache; the queries rotated in the same launch
+  kv4_read(cache, slots INT64[T], k, v)     cache rows back as the BF16 values they stand for
+  kv4_attention(q, cache, block_table INT32[B,W], q_starts INT32[B+1], kv_lens INT32[B], workspace, out, scale)
+      causal attention of single tokens and prompts; workspace UINT8[kv4_workspace_bytes()] zeroed once
+
 There is no CPU implementation and no fallback: if the compiled extension is missing the
 import fails, and the operators only have a CUDA kernel registered.
 """
@@ -65,6 +77,10 @@ dynamic_channel_mm = torch.ops.consumer_int8.dynamic_channel_mm
 fused_channel_mm_gather = torch.ops.consumer_int8.fused_channel_mm_gather
 fused_channel_mm_gather_sync = torch.ops.consumer_int8.fused_channel_mm_gather_sync
 peer_rendezvous = torch.ops.consumer_int8.peer_rendezvous
+qk_norm_rope = torch.ops.consumer_int8.qk_norm_rope
+kv4_append = torch.ops.consumer_int8.kv4_append
+kv4_read = torch.ops.consumer_int8.kv4_read
+kv4_attention = torch.ops.consumer_int8.kv4_attention
 
 
 @torch.library.register_fake("consumer_int8::fused_channel_mm")
@@ -152,3 +168,35 @@ def grouped_workspace_bytes(m: int, n: int, groups: int) -> int:
 @torch.library.register_fake("consumer_int8::grouped_channel_mm")
 def _grouped_channel_mm_fake(codes, w, scales, w_scale, out):
     return None
+
+
+@torch.library.register_fake("consumer_int8::qk_norm_rope")
+def _qk_norm_rope_fake(q, k, q_weight, k_weight, cos_sin, positions, axis_of, q_out, k_out, eps=1e-6, weight_offset=0.0, adjacent=False):
+    return None
+
+
+@torch.library.register_fake("consumer_int8::kv4_append")
+def _kv4_append_fake(q, k, v, cos_sin, positions, axis_of, slots, q_out, cache, adjacent=False):
+    return None
+
+
+@torch.library.register_fake("consumer_int8::kv4_read")
+def _kv4_read_fake(cache, slots, k, v):
+    return None
+
+
+@torch.library.register_fake("consumer_int8::kv4_attention")
+def _kv4_attention_fake(q, cache, block_table, q_starts, kv_lens, workspace, out, scale):
+    return None
+
+
+def kv4_block_bytes(page: int, dim: int) -> int:
+    """Last dimension of the 4-bit cache: the bytes that a page of one head's keys (or values) takes."""
+    return page * (dim // 2 + 4)
+
+
+def kv4_workspace_bytes() -> int:
+    """Bytes of (zero-initialised, UINT8) workspace that ``kv4_attention`` asks for, whatever the shapes. Calls that may
+    run at the same time need one each."""
+    libci8.ci8_kv4_workspace_bytes.restype = ctypes.c_longlong
+    return int(libci8.ci8_kv4_workspace_bytes())

@@ -11,6 +11,7 @@
 #include <torch/headeronly/util/Exception.h>
 #include <cstdint>
 #include <limits>
+#include <optional>
 #include "../../include/ci8.h"
 
 using torch::stable::Tensor;
@@ -393,6 +394,205 @@ void boxed_peer_rendezvous(StableIValue* stack, uint64_t, uint64_t) {
 }
 void boxed_fused_mm_gather(StableIValue* stack, uint64_t, uint64_t) { gather_common(stack, false); }
 void boxed_fused_mm_gather_sync(StableIValue* stack, uint64_t, uint64_t) { gather_common(stack, true); }
+
+// ---- the operators of the 4-bit key/value cache (include/ci8.h says what each computes) ----
+using OptionalTensor = std::optional<Tensor>;
+
+// A heads tensor [tokens, heads, dim]: the heads of a token are contiguous, tokens may be further apart (a
+// slice of a projection's output).
+struct Heads {
+  void* data;
+  int64_t tokens, heads, dim, stride;
+};
+Heads heads_of(const Tensor& t, int device) {
+  STD_TORCH_CHECK(t.is_cuda() && t.get_device_index() == device, "All tensors must be on the same CUDA device");
+  STD_TORCH_CHECK(t.scalar_type() == ScalarType::BFloat16 && t.dim() == 3, "Expected BF16 heads [tokens, heads, dim]");
+  Heads h{t.data_ptr(), t.size(0), t.size(1), t.size(2), t.size(1) * t.size(2)};
+  STD_TORCH_CHECK(h.dim == 64 || h.dim == 128 || h.dim == 256, "Head dimension must be 64, 128 or 256");
+  STD_TORCH_CHECK(h.heads > 0 && h.heads <= 1024 && h.tokens <= kIntMax, "Unsupported number of heads or tokens");
+  STD_TORCH_CHECK(t.stride(2) == 1 && (h.heads == 1 || t.stride(1) == h.dim), "The heads of a token must be contiguous");
+  if (h.tokens > 1) h.stride = t.stride(0);
+  STD_TORCH_CHECK(h.tokens == 0 || (h.stride >= h.heads * h.dim && h.stride % 8 == 0 && address(t) % 16 == 0),
+                  "Heads need 16-byte aligned rows that do not overlap");
+  return h;
+}
+// Whether two heads tensors share memory. Slices of one buffer (equal strides) may lie between one another.
+bool overlap(const Heads& a, const Heads& b) {
+  if (!a.tokens || !b.tokens) return false;
+  const int64_t first = reinterpret_cast<intptr_t>(a.data), second = reinterpret_cast<intptr_t>(b.data);
+  const int64_t width_a = 2 * a.heads * a.dim, width_b = 2 * b.heads * b.dim;
+  const int64_t end_a = first + 2 * (a.tokens - 1) * a.stride + width_a, end_b = second + 2 * (b.tokens - 1) * b.stride + width_b;
+  if (first >= end_b || second >= end_a) return false;
+  if (a.stride != b.stride) return true;
+  const int64_t stride = 2 * a.stride;
+  const int64_t offset = ((second - first) % stride + stride) % stride;   // of b's rows behind a's
+  return offset < width_a || offset + width_b > stride;
+}
+bool overlap(const Heads& a, const void* data, int64_t bytes) {
+  if (!a.tokens || !bytes) return false;
+  const int64_t first = reinterpret_cast<intptr_t>(a.data), second = reinterpret_cast<intptr_t>(data);
+  return first < second + bytes && second < first + 2 * ((a.tokens - 1) * a.stride + a.heads * a.dim);
+}
+bool same_rows(const Heads& a, const Heads& b) { return a.data == b.data && a.stride == b.stride; }
+
+struct Rotation {
+  const float* cos_sin = nullptr;
+  const int64_t* positions = nullptr;
+  const int32_t* axis_of = nullptr;
+  int table_rows = 0, rotary = 0, axes = 1;
+};
+Rotation rotation_of(const OptionalTensor& cos_sin, const OptionalTensor& positions, const OptionalTensor& axis_of, const Heads& k, int device) {
+  Rotation r;
+  if (!cos_sin.has_value()) {
+    STD_TORCH_CHECK(!positions.has_value() && !axis_of.has_value(), "positions and axis_of need a cos_sin table");
+    return r;
+  }
+  STD_TORCH_CHECK(positions.has_value(), "cos_sin needs positions");
+  check(*cos_sin, ScalarType::Float, device);
+  check(*positions, ScalarType::Long, device);
+  STD_TORCH_CHECK(cos_sin->dim() == 2 && cos_sin->size(0) > 0 && cos_sin->size(0) <= kIntMax && cos_sin->size(1) > 0 &&
+                      cos_sin->size(1) % 16 == 0 && cos_sin->size(1) <= k.dim && address(*cos_sin) % 16 == 0,
+                  "Expected an aligned FP32 cos_sin table [rows, rotary], rotary a multiple of 16 up to the head dimension");
+  const int64_t axes = positions->dim() == 2 ? positions->size(0) : 1;
+  STD_TORCH_CHECK((positions->dim() == 1 || positions->dim() == 2) && positions->size(positions->dim() - 1) == k.tokens && axes > 0 && axes <= 4,
+                  "Expected INT64 positions [tokens] or [axes, tokens], at most 4 axes");
+  STD_TORCH_CHECK(axis_of.has_value() || axes == 1, "Several position axes need axis_of");
+  if (axis_of.has_value()) {
+    check(*axis_of, ScalarType::Int, device);
+    STD_TORCH_CHECK(axis_of->dim() == 1 && axis_of->size(0) == cos_sin->size(1) / 2, "Expected INT32 axis_of [rotary / 2]");
+    r.axis_of = static_cast<const int32_t*>(axis_of->data_ptr());
+  }
+  r.cos_sin = static_cast<const float*>(cos_sin->data_ptr());
+  r.positions = static_cast<const int64_t*>(positions->data_ptr());
+  r.table_rows = static_cast<int>(cos_sin->size(0));
+  r.rotary = static_cast<int>(cos_sin->size(1));
+  r.axes = static_cast<int>(axes);
+  return r;
+}
+
+struct Cache {
+  void* data;
+  int64_t pages, heads, page, bytes;
+};
+Cache cache_of(const Tensor& t, int64_t dim, int64_t kv_heads, int device) {
+  check(t, ScalarType::Byte, device);
+  STD_TORCH_CHECK(t.dim() == 4 && t.size(1) == 2 && t.size(2) == kv_heads && t.size(0) <= kIntMax && t.size(3) % (dim / 2 + 4) == 0,
+                  "Expected a UINT8 cache [pages, 2, heads, page * (dim / 2 + 4)]");
+  Cache c{t.data_ptr(), t.size(0), t.size(2), t.size(3) / (dim / 2 + 4), t.numel()};
+  STD_TORCH_CHECK(c.page == 16 || c.page == 32 || c.page == 64 || c.page == 128 || c.page == 256, "Cache pages hold 16, 32, 64, 128 or 256 tokens");
+  STD_TORCH_CHECK(address(t) % 16 == 0, "The cache must be 16-byte aligned");
+  return c;
+}
+
+void boxed_qk_norm_rope(StableIValue* stack, uint64_t, uint64_t) {
+  auto q = to<Tensor>(stack[0]), k = to<Tensor>(stack[1]);
+  auto q_weight = to<OptionalTensor>(stack[2]), k_weight = to<OptionalTensor>(stack[3]);
+  auto cos_sin = to<OptionalTensor>(stack[4]), positions = to<OptionalTensor>(stack[5]), axis_of = to<OptionalTensor>(stack[6]);
+  auto q_out = to<Tensor>(stack[7]), k_out = to<Tensor>(stack[8]);
+  const double eps = to<double>(stack[9]), weight_offset = to<double>(stack[10]);
+  const bool adjacent = to<bool>(stack[11]);
+  const int device = q.get_device_index();
+  const Heads hq = heads_of(q, device), hk = heads_of(k, device), oq = heads_of(q_out, device), ok = heads_of(k_out, device);
+  STD_TORCH_CHECK(hq.tokens == hk.tokens && hq.dim == hk.dim && oq.tokens == hq.tokens && oq.heads == hq.heads && oq.dim == hq.dim &&
+                      ok.tokens == hk.tokens && ok.heads == hk.heads && ok.dim == hk.dim,
+                  "Wrong query, key or output shapes");
+  for (const OptionalTensor* w : {&q_weight, &k_weight}) {
+    if (!w->has_value()) continue;
+    check(**w, ScalarType::BFloat16, device);
+    STD_TORCH_CHECK((*w)->dim() == 1 && (*w)->size(0) == hq.dim && address(**w) % 16 == 0, "Expected an aligned BF16 norm weight [dim]");
+    STD_TORCH_CHECK(!overlap(oq, (*w)->data_ptr(), 2 * hq.dim) && !overlap(ok, (*w)->data_ptr(), 2 * hq.dim), "Outputs must not overlap the weights");
+  }
+  STD_TORCH_CHECK(eps >= 0, "eps must not be negative");
+  STD_TORCH_CHECK((same_rows(oq, hq) || !overlap(oq, hq)) && (same_rows(ok, hk) || !overlap(ok, hk)) && !overlap(oq, hk) &&
+                      !overlap(ok, hq) && !overlap(oq, ok),
+                  "An output may be its own input and must not overlap anything else");
+  const Rotation r = rotation_of(cos_sin, positions, axis_of, hk, device);
+  torch::stable::accelerator::DeviceGuard guard(device);
+  launched(ci8_qk_norm_rope(hq.data, hq.stride, hk.data, hk.stride, q_weight.has_value() ? q_weight->data_ptr() : nullptr,
+                            k_weight.has_value() ? k_weight->data_ptr() : nullptr, r.cos_sin, r.table_rows, r.rotary, r.positions, r.axes,
+                            r.axis_of, oq.data, oq.stride, ok.data, ok.stride, hq.tokens, hq.heads, hk.heads, hq.dim,
+                            static_cast<float>(eps), static_cast<float>(weight_offset), adjacent, stream_for(device)));
+}
+
+void boxed_kv4_append(StableIValue* stack, uint64_t, uint64_t) {
+  auto q = to<OptionalTensor>(stack[0]);
+  auto k = to<Tensor>(stack[1]), v = to<Tensor>(stack[2]);
+  auto cos_sin = to<OptionalTensor>(stack[3]), positions = to<OptionalTensor>(stack[4]), axis_of = to<OptionalTensor>(stack[5]);
+  auto slots = to<Tensor>(stack[6]);
+  auto q_out = to<OptionalTensor>(stack[7]);
+  auto cache = to<Tensor>(stack[8]);
+  const bool adjacent = to<bool>(stack[9]);
+  const int device = k.get_device_index();
+  const Heads hk = heads_of(k, device), hv = heads_of(v, device);
+  STD_TORCH_CHECK(hv.tokens == hk.tokens && hv.heads == hk.heads && hv.dim == hk.dim, "Wrong key or value shapes");
+  check(slots, ScalarType::Long, device);
+  STD_TORCH_CHECK(slots.dim() == 1 && slots.size(0) == hk.tokens, "Expected INT64 slots [tokens]");
+  const Cache c = cache_of(cache, hk.dim, hk.heads, device);
+  STD_TORCH_CHECK(q.has_value() == q_out.has_value(), "q and q_out come together");
+  STD_TORCH_CHECK(!overlap(hk, c.data, c.bytes) && !overlap(hv, c.data, c.bytes), "The cache must not overlap the inputs");
+  Heads hq{}, oq{};
+  if (q.has_value()) {
+    hq = heads_of(*q, device);
+    oq = heads_of(*q_out, device);
+    STD_TORCH_CHECK(hq.tokens == hk.tokens && hq.dim == hk.dim && oq.tokens == hq.tokens && oq.heads == hq.heads && oq.dim == hq.dim,
+                    "Wrong query shapes");
+    STD_TORCH_CHECK((same_rows(oq, hq) || !overlap(oq, hq)) && !overlap(oq, hk) && !overlap(oq, hv) && !overlap(oq, c.data, c.bytes) &&
+                        !overlap(hq, c.data, c.bytes),
+                    "q_out may be q and must not overlap anything else");
+  }
+  const Rotation r = rotation_of(cos_sin, positions, axis_of, hk, device);
+  torch::stable::accelerator::DeviceGuard guard(device);
+  launched(ci8_kv4_append(hq.data, hq.stride, hk.data, hk.stride, hv.data, hv.stride, r.cos_sin, r.table_rows, r.rotary, r.positions,
+                          r.axes, r.axis_of, static_cast<const int64_t*>(slots.data_ptr()), oq.data, oq.stride, c.data, c.pages, c.page,
+                          hk.tokens, hq.heads, hk.heads, hk.dim, adjacent, stream_for(device)));
+}
+
+void boxed_kv4_read(StableIValue* stack, uint64_t, uint64_t) {
+  auto cache = to<Tensor>(stack[0]), slots = to<Tensor>(stack[1]), k = to<Tensor>(stack[2]), v = to<Tensor>(stack[3]);
+  const int device = cache.get_device_index();
+  const Heads hk = heads_of(k, device), hv = heads_of(v, device);
+  STD_TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && hv.tokens == hk.tokens && hv.heads == hk.heads && hv.dim == hk.dim,
+                  "Expected contiguous keys and values of one shape");
+  check(slots, ScalarType::Long, device);
+  STD_TORCH_CHECK(slots.dim() == 1 && slots.size(0) == hk.tokens, "Expected INT64 slots [tokens]");
+  const Cache c = cache_of(cache, hk.dim, hk.heads, device);
+  STD_TORCH_CHECK(!overlap(hk, hv) && !overlap(hk, c.data, c.bytes) && !overlap(hv, c.data, c.bytes) &&
+                      !overlap(hk, slots.data_ptr(), 8 * hk.tokens) && !overlap(hv, slots.data_ptr(), 8 * hk.tokens),
+                  "Outputs must not overlap anything else");
+  torch::stable::accelerator::DeviceGuard guard(device);
+  launched(ci8_kv4_read(c.data, static_cast<const int64_t*>(slots.data_ptr()), hk.data, hv.data, c.pages, c.page, hk.tokens, hk.heads,
+                        hk.dim, stream_for(device)));
+}
+
+void boxed_kv4_attention(StableIValue* stack, uint64_t, uint64_t) {
+  auto q = to<Tensor>(stack[0]), cache = to<Tensor>(stack[1]), block_table = to<Tensor>(stack[2]), q_starts = to<Tensor>(stack[3]);
+  auto kv_lens = to<Tensor>(stack[4]), workspace = to<Tensor>(stack[5]), out = to<Tensor>(stack[6]);
+  const double scale = to<double>(stack[7]);
+  const int device = q.get_device_index();
+  const Heads hq = heads_of(q, device), ho = heads_of(out, device);
+  STD_TORCH_CHECK(out.is_contiguous() && ho.tokens == hq.tokens && ho.heads == hq.heads && ho.dim == hq.dim, "Wrong output shape");
+  STD_TORCH_CHECK(cache.dim() == 4 && cache.size(2) > 0 && hq.heads % cache.size(2) == 0, "The query heads must be a multiple of the cache's heads");
+  const Cache c = cache_of(cache, hq.dim, cache.size(2), device);
+  check(block_table, ScalarType::Int, device);
+  check(q_starts, ScalarType::Int, device);
+  check(kv_lens, ScalarType::Int, device);
+  check(workspace, ScalarType::Byte, device);
+  STD_TORCH_CHECK(kv_lens.dim() == 1 && block_table.dim() == 2 && block_table.size(0) == kv_lens.size(0) && q_starts.dim() == 1 &&
+                      q_starts.size(0) == kv_lens.size(0) + 1 && block_table.numel() <= kIntMax && block_table.size(1) * c.page <= kIntMax,
+                  "Expected INT32 block_table [batch, width], q_starts [batch + 1] and kv_lens [batch]");
+  STD_TORCH_CHECK(workspace.numel() >= ci8_kv4_workspace_bytes() && address(workspace) % 16 == 0,
+                  "The attention workspace is too small or not aligned");
+  STD_TORCH_CHECK(scale > 0 && scale < 3.0e38, "The softmax scale must be positive and finite");
+  STD_TORCH_CHECK(!overlap(ho, hq) && !overlap(ho, c.data, c.bytes) && !overlap(ho, workspace.data_ptr(), workspace.numel()) &&
+                      !overlap(hq, workspace.data_ptr(), workspace.numel()) && !overlap(ho, block_table.data_ptr(), 4 * block_table.numel()) &&
+                      !overlap(ho, q_starts.data_ptr(), 4 * q_starts.numel()) && !overlap(ho, kv_lens.data_ptr(), 4 * kv_lens.numel()),
+                  "out and workspace must not overlap anything else");
+  torch::stable::accelerator::DeviceGuard guard(device);
+  launched(ci8_kv4_attention(hq.data, hq.stride, c.data, static_cast<const int32_t*>(block_table.data_ptr()),
+                             static_cast<const int32_t*>(q_starts.data_ptr()), static_cast<const int32_t*>(kv_lens.data_ptr()),
+                             workspace.data_ptr(), ho.data, hq.tokens, kv_lens.size(0), block_table.size(1), c.pages, c.page, hq.heads,
+                             c.heads, hq.dim, static_cast<float>(scale), stream_for(device)));
+}
 }  // namespace
 
 STABLE_TORCH_LIBRARY(consumer_int8, m) {
@@ -412,6 +612,10 @@ STABLE_TORCH_LIBRARY(consumer_int8, m) {
   m.def("fused_channel_mm_gather(Tensor a, Tensor w, Tensor a_scale, Tensor w_scale, Tensor(a!) gathered, Tensor peer_ptrs, int rank, int schedule=0) -> ()");
   m.def("peer_rendezvous(Tensor signal_ptrs, Tensor(a!) state, int rank) -> ()");
   m.def("fused_channel_mm_gather_sync(Tensor a, Tensor w, Tensor a_scale, Tensor w_scale, Tensor(a!) gathered, Tensor peer_ptrs, Tensor signal_ptrs, Tensor(b!) state, int rank, int schedule=0) -> ()");
+  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? cos_sin, Tensor? positions, Tensor? axis_of, Tensor(a!) q_out, Tensor(b!) k_out, float eps=1e-06, float weight_offset=0.0, bool adjacent=False) -> ()");
+  m.def("kv4_append(Tensor? q, Tensor k, Tensor v, Tensor? cos_sin, Tensor? positions, Tensor? axis_of, Tensor slots, Tensor(a!)? q_out, Tensor(b!) cache, bool adjacent=False) -> ()");
+  m.def("kv4_read(Tensor cache, Tensor slots, Tensor(a!) k, Tensor(b!) v) -> ()");
+  m.def("kv4_attention(Tensor q, Tensor cache, Tensor block_table, Tensor q_starts, Tensor kv_lens, Tensor(a!) workspace, Tensor(b!) out, float scale) -> ()");
 }
 STABLE_TORCH_LIBRARY_IMPL(consumer_int8, CUDA, m) {
   m.impl("silu_mul", &boxed_silu_mul);
@@ -430,6 +634,10 @@ STABLE_TORCH_LIBRARY_IMPL(consumer_int8, CUDA, m) {
   m.impl("fused_channel_mm_gather", &boxed_fused_mm_gather);
   m.impl("fused_channel_mm_gather_sync", &boxed_fused_mm_gather_sync);
   m.impl("peer_rendezvous", &boxed_peer_rendezvous);
+  m.impl("qk_norm_rope", &boxed_qk_norm_rope);
+  m.impl("kv4_append", &boxed_kv4_append);
+  m.impl("kv4_read", &boxed_kv4_read);
+  m.impl("kv4_attention", &boxed_kv4_attention);
 }
 extern "C" PyObject* PyInit__C() {
   static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_C", nullptr, -1, nullptr};

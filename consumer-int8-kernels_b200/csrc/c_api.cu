@@ -14,6 +14,8 @@
 #include "decode_splitk.cuh"
 #include "gemm_tcgen05.cuh"
 #include "gemv_w8a16.cuh"
+#include "kv4_attention.cuh"
+#include "kv4_rows.cuh"
 #include "q8_block.cuh"
 #include "quantize.cuh"
 
@@ -800,6 +802,69 @@ cudaError_t q8_static_scratch(unsigned char** out) {
   return cudaSuccess;
 }
 
+namespace {
+// ------------------------------------------------------------------ 4-bit key/value cache
+// Launch with programmatic stream serialization: every kernel below starts with griddepcontrol.wait.
+template <typename Params>
+int launch_pdl(void (*kernel)(Params), dim3 grid, int threads, size_t smem, ci8_stream_t stream, const Params& params) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = reinterpret_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&config, kernel, params));
+}
+
+constexpr int kKv4MaxHeads = 1024;
+constexpr long long kKv4WorkspaceBytes = 48ll << 20;
+bool kv4_dim(int dim) { return dim == 64 || dim == 128 || dim == 256; }
+// log2 of a page size the cache may have, -1 otherwise
+int kv4_page_shift(int page) {
+  for (int shift = 4; shift <= 8; ++shift)
+    if (page == 1 << shift) return shift;
+  return -1;
+}
+bool kv4_row_source(const void* p, long long stride, int tokens, int heads, int dim) {
+  return p && aligned(p, 16) && stride % 8 == 0 && (tokens <= 1 || stride >= static_cast<long long>(heads) * dim);
+}
+bool kv4_rotation(const float* cos_sin, int table_rows, int rotary, const int64_t* positions, int axes, const int32_t* axis_of, int dim) {
+  if (!cos_sin) return true;
+  return aligned(cos_sin, 16) && table_rows > 0 && rotary > 0 && rotary % 16 == 0 && rotary <= dim && positions && aligned(positions, 8) &&
+         axes > 0 && axes <= 4 && aligned(axis_of, 4) && (axis_of || axes == 1);
+}
+
+// Heads of a token go to one warp while there are tokens enough to fill the GPU with four batches of loads per
+// warp, and are cut into single batches otherwise (a generated token: 28 heads of 256 components on 28 warps
+// instead of 1).
+template <int kDim, bool kNorm, bool kAppend>
+int launch_kv4_rows(Kv4RowParams p, ci8_stream_t stream) {
+  const int per_step = 32 / (kDim / 8);
+  const int heads = (p.q ? p.q_heads : 0) + p.kv_heads * (kAppend ? 2 : 1);
+  const long long steps = (heads + per_step - 1) / per_step;
+  const long long busy = static_cast<long long>(sm_count()) * 32;
+  long long chunks = (busy + p.tokens - 1) / p.tokens;
+  if (chunks > steps) chunks = steps;
+  const long long four = (steps + 3) / 4;
+  if (chunks < four) chunks = four;
+  const long long per_chunk = ((steps + chunks - 1) / chunks) * per_step;
+  p.chunks = static_cast<int>((heads + per_chunk - 1) / per_chunk);
+  const long long warps = static_cast<long long>(p.tokens) * p.chunks;
+  const int per_cta = warps < 4 * sm_count() ? 1 : 8;
+  return launch_pdl(kv4_rows_kernel<kDim, kNorm, kAppend>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
+}
+template <bool kNorm, bool kAppend>
+int launch_kv4_rows(const Kv4RowParams& p, int dim, ci8_stream_t stream) {
+  return dim == 64 ? launch_kv4_rows<64, kNorm, kAppend>(p, stream)
+         : dim == 128 ? launch_kv4_rows<128, kNorm, kAppend>(p, stream) : launch_kv4_rows<256, kNorm, kAppend>(p, stream);
+}
+
+}  // namespace
+
 // ====================================================================== C ABI
 extern "C" {
 
@@ -1181,6 +1246,98 @@ int ci8_decode_mm_split(const int8_t* a, const void* w, const float* a_scale, co
                  workspace, m, n, k, 0};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return weights_biased ? launch_decode<true>(a, w, p, split, s) : launch_decode<false>(a, w, p, split, s);
+}
+
+int ci8_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride, const void* q_weight,
+                     const void* k_weight, const float* cos_sin, int table_rows, int rotary, const int64_t* positions,
+                     int axes, const int32_t* axis_of, void* q_out, long long q_out_stride, void* k_out,
+                     long long k_out_stride, int tokens, int q_heads, int kv_heads, int dim, float eps,
+                     float weight_offset, int adjacent, ci8_stream_t stream) {
+  if (tokens < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > kKv4MaxHeads || kv_heads > kKv4MaxHeads || !kv4_dim(dim)) return kInvalid;
+  if (tokens == 0) return 0;
+  if (!kv4_row_source(q, q_stride, tokens, q_heads, dim) || !kv4_row_source(k, k_stride, tokens, kv_heads, dim) ||
+      !kv4_row_source(q_out, q_out_stride, tokens, q_heads, dim) || !kv4_row_source(k_out, k_out_stride, tokens, kv_heads, dim) ||
+      !aligned(q_weight, 16) || !aligned(k_weight, 16) || !(eps >= 0.f) ||
+      !kv4_rotation(cos_sin, table_rows, rotary, positions, axes, axis_of, dim))
+    return kInvalid;
+  Kv4RowParams p = {};
+  p.q = static_cast<const uint16_t*>(q); p.k = static_cast<const uint16_t*>(k);
+  p.q_out = static_cast<uint16_t*>(q_out); p.k_out = static_cast<uint16_t*>(k_out);
+  p.q_stride = q_stride; p.k_stride = k_stride; p.q_out_stride = q_out_stride; p.k_out_stride = k_out_stride;
+  p.q_weight = static_cast<const uint16_t*>(q_weight); p.k_weight = static_cast<const uint16_t*>(k_weight);
+  p.cos_sin = cos_sin; p.positions = positions; p.axis_of = axis_of;
+  p.table_rows = table_rows; p.rotary = cos_sin ? rotary : 0; p.axes = axes; p.adjacent = adjacent != 0;
+  p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.eps = eps; p.weight_offset = weight_offset;
+  return launch_kv4_rows<true, false>(p, dim, stream);
+}
+
+int ci8_kv4_append(const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
+                   const float* cos_sin, int table_rows, int rotary, const int64_t* positions, int axes,
+                   const int32_t* axis_of, const int64_t* slots, void* q_out, long long q_out_stride, void* cache,
+                   int pages, int page, int tokens, int q_heads, int kv_heads, int dim, int adjacent, ci8_stream_t stream) {
+  const int shift = kv4_page_shift(page);
+  if (tokens < 0 || (q && (q_heads <= 0 || q_heads > kKv4MaxHeads)) || kv_heads <= 0 || kv_heads > kKv4MaxHeads || !kv4_dim(dim) ||
+      shift < 0 || pages < 0)
+    return kInvalid;
+  if (tokens == 0) return 0;
+  if ((q && (!kv4_row_source(q, q_stride, tokens, q_heads, dim) || !kv4_row_source(q_out, q_out_stride, tokens, q_heads, dim))) ||
+      !kv4_row_source(k, k_stride, tokens, kv_heads, dim) || !kv4_row_source(v, v_stride, tokens, kv_heads, dim) ||
+      !slots || !aligned(slots, 8) || !cache || !aligned(cache, 16) ||
+      !kv4_rotation(cos_sin, table_rows, rotary, positions, axes, axis_of, dim))
+    return kInvalid;
+  Kv4RowParams p = {};
+  p.q = static_cast<const uint16_t*>(q); p.k = static_cast<const uint16_t*>(k); p.v = static_cast<const uint16_t*>(v);
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride; p.q_out_stride = q_out_stride;
+  p.cos_sin = cos_sin; p.positions = positions; p.axis_of = axis_of; p.slots = slots;
+  p.cache = static_cast<uint8_t*>(cache); p.capacity = static_cast<int64_t>(pages) << shift;
+  p.table_rows = table_rows; p.rotary = cos_sin ? rotary : 0; p.axes = axes; p.adjacent = adjacent != 0;
+  p.tokens = tokens; p.q_heads = q ? q_heads : 0; p.kv_heads = kv_heads; p.page_shift = shift;
+  return launch_kv4_rows<false, true>(p, dim, stream);
+}
+
+int ci8_kv4_read(const void* cache, const int64_t* slots, void* k, void* v, int pages, int page, int tokens, int kv_heads,
+                 int dim, ci8_stream_t stream) {
+  const int shift = kv4_page_shift(page);
+  if (tokens < 0 || kv_heads <= 0 || kv_heads > kKv4MaxHeads || !kv4_dim(dim) || shift < 0 || pages < 0) return kInvalid;
+  if (tokens == 0) return 0;
+  if (!cache || !aligned(cache, 16) || !slots || !aligned(slots, 8) || !k || !v || !aligned(k, 16) || !aligned(v, 16)) return kInvalid;
+  Kv4ReadParams p = {};
+  p.cache = static_cast<const uint8_t*>(cache); p.slots = slots;
+  p.k = static_cast<uint16_t*>(k); p.v = static_cast<uint16_t*>(v);
+  p.capacity = static_cast<int64_t>(pages) << shift; p.rows = static_cast<int64_t>(tokens) * 2 * kv_heads;
+  p.kv_heads = kv_heads; p.page_shift = shift;
+  const int64_t per_cta = 256 / (dim / 8);
+  int64_t grid = (p.rows + per_cta - 1) / per_cta;
+  const int64_t most = static_cast<int64_t>(sm_count()) * 8;
+  if (grid > most) grid = most;
+  return dim == 64 ? launch_pdl(kv4_read_kernel<64>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p)
+         : dim == 128 ? launch_pdl(kv4_read_kernel<128>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p)
+                      : launch_pdl(kv4_read_kernel<256>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p);
+}
+
+long long ci8_kv4_workspace_bytes(void) { return kKv4WorkspaceBytes; }
+
+int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, const int32_t* block_table, const int32_t* q_starts,
+                      const int32_t* kv_lens, void* workspace, void* out, int tokens, int batch, int width, int pages, int page,
+                      int q_heads, int kv_heads, int dim, float scale, ci8_stream_t stream) {
+  const int shift = kv4_page_shift(page);
+  if (tokens < 0 || batch < 0 || width < 0 || pages < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > kKv4MaxHeads ||
+      q_heads % kv_heads || !kv4_dim(dim) || shift < 0 || !(scale > 0.f) || !(scale < 3.0e38f))
+    return kInvalid;
+  if (tokens == 0 || batch == 0) return 0;
+  if (!kv4_row_source(q, q_stride, tokens, q_heads, dim) || (pages > 0 && !cache) || !aligned(cache, 16) || (width > 0 && !block_table) ||
+      !aligned(block_table, 4) || !q_starts || !aligned(q_starts, 4) || !kv_lens || !aligned(kv_lens, 4) || !workspace ||
+      !aligned(workspace, 16) || !out || !aligned(out, 16) || (static_cast<long long>(width) << shift) > 0x7fffffffll)
+    return kInvalid;
+  Kv4AttendParams p = {};
+  p.q = static_cast<const uint16_t*>(q); p.q_stride = q_stride; p.cache = static_cast<const uint8_t*>(cache);
+  p.block_table = block_table; p.q_starts = q_starts; p.kv_lens = kv_lens; p.out = static_cast<uint16_t*>(out);
+  p.tokens = tokens; p.batch = batch; p.width = width; p.q_heads = q_heads; p.kv_heads = kv_heads;
+  p.page_shift = shift; p.pages = pages; p.scale_log2 = scale * 1.4426950408889634f;
+  const dim3 grid(tokens, q_heads);
+  return dim == 64 ? launch_pdl(kv4_attend_kernel<64>, grid, 128, 0, stream, p)
+         : dim == 128 ? launch_pdl(kv4_attend_kernel<128>, grid, 128, 0, stream, p) : launch_pdl(kv4_attend_kernel<256>, grid, 128, 0, stream, p);
 }
 
 }  // extern "C"

@@ -214,6 +214,67 @@ int ci8_fused_channel_mm_gather_sync(const int8_t* a, const int8_t* w, const flo
  * with that entry point). Bounded like every wait: 2 s, then status bit 2. */
 int ci8_peer_rendezvous(void* const* signals, void* state, int world, int rank, ci8_stream_t stream);
 
+/* ---- Attention side of the layer, over a key/value cache held in 4 bits (no counterpart behind this header's
+ * other entry points; the row format is this library's own) ----
+ *
+ * Cache: UINT8 [pages, 2 (0 keys, 1 values), kv_heads, page * (dim / 2 + 4)], 16-byte aligned; page = 16, 32, 64,
+ * 128 or 256 tokens, dim = 64, 128 or 256. The block of (page, side, head) holds `page` rows of dim / 2 bytes
+ * (byte j: component 2j in the low and 2j + 1 in the high four bits), then `page` pairs of BF16 numbers (scale,
+ * zero point); a code c stands for scale * (c - zero). Slot s of the cache is row s % page of page s / page.
+ *
+ * Heads tensors are BF16 [tokens, heads, dim] with a token stride given in elements (a multiple of 8), 16-byte
+ * aligned, so that slices of one projection's output can be passed. Head counts up to 1024.
+ *
+ * A position, slot or page number outside its table never leads to an access outside a buffer: the access is left
+ * out as described below and status bit 3 (value 8) is raised (ci8_device_status). */
+
+/* RMS norm of every query and key head and rotation to its position, in one launch:
+ *   y = x / sqrt(mean(x^2) + eps) * (weight + weight_offset)     skipped for a side whose weight is NULL
+ *   (a, b) -> (a cos - b sin, b cos + a sin)                     skipped when cos_sin is NULL
+ * over the first `rotary` components (a multiple of 16, <= dim): pairs (i, i + rotary/2), or (2i, 2i + 1) when
+ * `adjacent`; pair i takes cos_sin[position, i] and cos_sin[position, rotary/2 + i], cos_sin FP32 [table_rows,
+ * rotary]. positions INT64 [axes, tokens], axes <= 4; pair i uses the position on axis axis_of[i] (INT32
+ * [rotary/2]; NULL: one axis). Weights BF16 [dim]. FP32 inside, one rounding. An output may be its own input
+ * (same pointer and stride) and must not overlap any other argument. A token with a position outside the table
+ * or an axis outside 0..axes-1 is written as NaN. tokens == 0 is a no-op. */
+int ci8_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride, const void* q_weight,
+                     const void* k_weight, const float* cos_sin, int table_rows, int rotary, const int64_t* positions,
+                     int axes, const int32_t* axis_of, void* q_out, long long q_out_stride, void* k_out,
+                     long long k_out_stride, int tokens, int q_heads, int kv_heads, int dim, float eps,
+                     float weight_offset, int adjacent, ci8_stream_t stream);
+
+/* Appends keys and values to the cache: keys are rotated as above (not when cos_sin is NULL), then every key and
+ * value head is encoded: low = min(x, 0), high = max(x, 0) over the head, scale = bf16((high - low) / 15), at least
+ * 1e-20, zero = rint(-low / scale), code = clamp(rint(x / scale) + zero, 0, 15), IEEE divisions, halves to even.
+ * NaN counts as 0, infinities as +-8.5e37. q (NULL: none) is rotated into q_out in the same launch. slots INT64
+ * [tokens]: where each token goes; a negative slot is not stored (padding; its query is still rotated), nor is one
+ * beyond the cache or a token with a bad position (status bit 3). Slots that are stored must differ: two tokens
+ * with the same slot leave a mixture of both in it. */
+int ci8_kv4_append(const void* q, long long q_stride, const void* k, long long k_stride, const void* v, long long v_stride,
+                   const float* cos_sin, int table_rows, int rotary, const int64_t* positions, int axes,
+                   const int32_t* axis_of, const int64_t* slots, void* q_out, long long q_out_stride, void* cache,
+                   int pages, int page, int tokens, int q_heads, int kv_heads, int dim, int adjacent, ci8_stream_t stream);
+
+/* The cache rows of slots INT64 [tokens] as the values they stand for, BF16 k and v [tokens, kv_heads, dim]; zeros
+ * for a negative slot, and for one beyond the cache (status bit 3). */
+int ci8_kv4_read(const void* cache, const int64_t* slots, void* k, void* v, int pages, int page, int tokens, int kv_heads,
+                 int dim, ci8_stream_t stream);
+
+/* Bytes of device memory ci8_kv4_attention asks for, whatever the shapes. Zeroed once by the caller; every call leaves
+ * it fit for the next. Calls that may run at the same time need one each. */
+long long ci8_kv4_workspace_bytes(void);
+
+/* Causal attention over the cache. Sequence b owns the token rows q_starts[b] .. q_starts[b+1]-1 (INT32 [batch+1],
+ * ascending) of q and out, and the first kv_lens[b] (INT32) tokens of the pages block_table[b] (INT32 [batch, width])
+ * names, the last of which are its own rows' (already appended): row i of n sees the first kv_lens[b] - n + i + 1
+ * tokens. out = softmax(scale * q k^T) v, BF16 [tokens, q_heads, dim] contiguous; q_heads is a multiple of kv_heads,
+ * scale > 0. Rows that see nothing are zeros; rows of no sequence are left as they were. Lengths are cut to the
+ * table's width; tokens of a page number outside the cache are not seen (status bit 3), and entries behind a
+ * sequence's last page are not read. All lengths are read on the device, so a captured call follows their values. */
+int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, const int32_t* block_table, const int32_t* q_starts,
+                      const int32_t* kv_lens, void* workspace, void* out, int tokens, int batch, int width, int pages, int page,
+                      int q_heads, int kv_heads, int dim, float scale, ci8_stream_t stream);
+
 /* The streaming (m <= 64) kernel behind ci8_fused_channel_mm / ci8_cutlass_channel_mm /
  * ci8_channel_mm with the split-K factor forced to 1, 2 or 4 (1 or 2 for m > 16) instead of chosen
  * from the shape.
@@ -250,7 +311,8 @@ int ci8_selftest_cluster_timeout(unsigned deadline_us, int* gave_up, ci8_stream_
 /* Reads and clears the current device's kernel status word (synchronises the device). Bit 0: a
  * bounded wait inside a kernel ran past its deadline and the kernel gave up (its output is then
  * undefined); bit 1: a cluster rendezvous did; bit 2: the cross-GPU rendezvous of
- * ci8_fused_channel_mm_gather_sync did (a peer never arrived). Returns 0 or a cudaError_t. Not for use during stream capture. */
+ * ci8_fused_channel_mm_gather_sync did (a peer never arrived); bit 3: an operator of the 4-bit cache met a
+ * position, slot or page number outside its table and left that access out. Returns 0 or a cudaError_t. Not for use during stream capture. */
 int ci8_device_status(unsigned* status);
 
 /* The same check without a synchronisation, for serving loops that replay CUDA graphs (no counterpart in
