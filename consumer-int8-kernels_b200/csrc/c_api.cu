@@ -16,6 +16,7 @@
 #include "gemv_w8a16.cuh"
 #include "kv4_attention.cuh"
 #include "kv4_rows.cuh"
+#include "kv4_single.cuh"
 #include "q8_block.cuh"
 #include "quantize.cuh"
 
@@ -863,6 +864,29 @@ int launch_kv4_rows(const Kv4RowParams& p, int dim, ci8_stream_t stream) {
          : dim == 128 ? launch_kv4_rows<128, kNorm, kAppend>(p, stream) : launch_kv4_rows<256, kNorm, kAppend>(p, stream);
 }
 
+// Generated tokens: eight query rows per warp, or sixteen where a key head has more query heads than eight.
+template <int kDim, int kQ>
+int launch_kv4_single_q(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
+  using Cfg = Kv4SingleConfig<kDim, kQ>;
+  static std::atomic<uint64_t> raised{0};
+  const cudaError_t err = ensure_smem(kv4_single_kernel<kDim, kQ>, Cfg::kSmemBytes, raised);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  long long ctas = sm_count();
+  if (ctas > kKv4MaxCtas) ctas = kKv4MaxCtas;
+  while (kv4_single_workspace<kDim, kQ>(ctas) > kKv4WorkspaceBytes) --ctas;
+  Kv4SingleParams p;
+  p.a = a;
+  p.counters = static_cast<unsigned*>(workspace);
+  p.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv4CounterBytes);
+  p.most_rows = most_rows;
+  return launch_pdl(kv4_single_kernel<kDim, kQ>, dim3(static_cast<unsigned>(ctas)), Cfg::kWarps * 32, Cfg::kSmemBytes, stream, p);
+}
+template <int kDim>
+int launch_kv4_single(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
+  return a.q_heads / a.kv_heads <= 8 ? launch_kv4_single_q<kDim, 1>(a, workspace, most_rows, stream)
+                                     : launch_kv4_single_q<kDim, 2>(a, workspace, most_rows, stream);
+}
+
 }  // namespace
 
 // ====================================================================== C ABI
@@ -1335,9 +1359,8 @@ int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, cons
   p.block_table = block_table; p.q_starts = q_starts; p.kv_lens = kv_lens; p.out = static_cast<uint16_t*>(out);
   p.tokens = tokens; p.batch = batch; p.width = width; p.q_heads = q_heads; p.kv_heads = kv_heads;
   p.page_shift = shift; p.pages = pages; p.scale_log2 = scale * 1.4426950408889634f;
-  const dim3 grid(tokens, q_heads);
-  return dim == 64 ? launch_pdl(kv4_attend_kernel<64>, grid, 128, 0, stream, p)
-         : dim == 128 ? launch_pdl(kv4_attend_kernel<128>, grid, 128, 0, stream, p) : launch_pdl(kv4_attend_kernel<256>, grid, 128, 0, stream, p);
+  return dim == 64 ? launch_kv4_single<64>(p, workspace, 0x7fffffff, stream)
+         : dim == 128 ? launch_kv4_single<128>(p, workspace, 0x7fffffff, stream) : launch_kv4_single<256>(p, workspace, 0x7fffffff, stream);
 }
 
 }  // extern "C"
