@@ -1359,6 +1359,7 @@ int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, cons
   p.block_table = block_table; p.q_starts = q_starts; p.kv_lens = kv_lens; p.out = static_cast<uint16_t*>(out);
   p.tokens = tokens; p.batch = batch; p.width = width; p.q_heads = q_heads; p.kv_heads = kv_heads;
   p.page_shift = shift; p.pages = pages; p.scale_log2 = scale * 1.4426950408889634f;
+  p.group = Kv4Divisor::of(static_cast<unsigned>(q_heads / kv_heads));
   return dim == 64 ? launch_kv4_single<64>(p, workspace, 0x7fffffff, stream)
          : dim == 128 ? launch_kv4_single<128>(p, workspace, 0x7fffffff, stream) : launch_kv4_single<256>(p, workspace, 0x7fffffff, stream);
 }

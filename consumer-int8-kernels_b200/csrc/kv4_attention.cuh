@@ -4,6 +4,18 @@
 
 namespace ci8 {
 
+// Division by a number that is known on the host: n / d for n below 2^31 as a product and a shift (m is
+// 2^(31 + s) / d rounded up, s = ceil(log2 d), so the error n * (m - 2^(31+s)/d) / 2^(31+s) stays below 1 / d).
+struct Kv4Divisor {
+  unsigned m, s, d;
+  __host__ static Kv4Divisor of(unsigned d) {
+    unsigned s = 0;
+    while ((1ull << s) < d) ++s;
+    return {static_cast<unsigned>(((1ull << (31 + s)) + d - 1) / d), s, d};
+  }
+  __device__ __forceinline__ int quotient(int n) const { return static_cast<int>(__umulhi(2u * static_cast<unsigned>(n), m) >> s); }
+};
+
 struct Kv4AttendParams {
   const uint16_t* q;          // [tokens, q_heads, dim], token stride in elements
   int64_t q_stride;
@@ -14,6 +26,7 @@ struct Kv4AttendParams {
   uint16_t* out;              // [tokens, q_heads, dim]
   int tokens, batch, width, q_heads, kv_heads, page_shift, pages;
   float scale_log2;           // softmax scale * log2(e)
+  Kv4Divisor group;           // query heads per key head
 };
 
 // The rows and keys of sequence b, with whatever the metadata says cut to the tensors' sizes.

@@ -3,18 +3,24 @@
 //
 // Work is cut into tiles of 32 tokens of one (sequence, key head, block of query rows) and the tiles of all of them,
 // laid end to end, are dealt to the warps in equal contiguous ranges, so that ragged batches fill the GPU evenly and
-// a long history is split as far as there are warps. Every warp runs on its own: its ring of tiles is filled by bulk
-// copies it issues itself, and it keeps its own running maximum, sum and output. Ranges begin and end inside a
+// a long history is split as far as there are warps. Every warp runs on its own: its ring of tiles is filled by
+// asynchronous copies it issues itself, and it keeps its own running maximum, sum and output. Ranges begin and end inside a
 // sequence; what a warp has of such a sequence is joined with its neighbours' inside the CTA at the end, and across
 // CTAs by whichever of them comes last, in the order of the CTAs (so the bits do not depend on the timing).
 //
-// The products run transposed on the tensor cores with register-fed operands: S^T[token, query] = K Q^T and
-// O^T[component, query] = V^T P^T (mma.sync m16n8k16), so that eight query rows fill an instruction and the cache is
-// the operand that is unpacked on the way, straight from its packed words: four bits become the BF16 number
-// 128 + code by one mask-and-or. Keys keep the 128 (it is taken out of the score, exactly scaled, as
-// (128 + zero) * sum of q); values are made exact small integers code - zero by one packed subtraction, because
-// their products are summed over the whole history. The values' scales go into the weights before they are rounded
-// to BF16 for the second product (2^-9 relative each, the size of the output's own rounding); all else is FP32.
+// The products run transposed on the tensor cores with register-fed operands (mma.sync), S^T[token, query] = K Q^T and
+// O^T[component, query] = V^T P^T, so that eight query rows fill an instruction and the cache is the operand that is
+// unpacked on the way, straight from its packed words. What limits the kernel beside the memory is the logic pipe
+// (two cycles a mask-and-or), so each product takes the form that needs the fewest:
+//   S^T  INT8 (m16n8k32): two masks give the eight codes of a word. The queries become 16-bit fixed point, two INT8
+//        digits relative to the row's largest component, two exact integer products; a query component is off by at
+//        most 2^-17 of the largest, a score of BF16 queries whose components lie within a factor 128 by less than the
+//        queries' own rounding. The sums, less zero * sum of q, stay exact until the key's scale is applied in FP32.
+//   O^T  FP16 (m16n8k16): a mask-and-or gives 1024 + code or 1024 + 16 * code for two tokens, one packed FMA the exact
+//        small integer code - zero (not zero points taken out of the sum afterwards: a sum over the whole history
+//        would cancel). The weights carry the values' scales, relative to the largest scale so far, which keeps them
+//        within FP16: full precision down to 2^-21 of the largest, 2^-11 relative rounding.
+// Maxima, sums, scores and outputs are FP32.
 #pragma once
 #include "kv4_attention.cuh"
 
@@ -52,15 +58,28 @@ struct Kv4SingleParams {
   int most_rows;              // sequences with more query rows (rows * heads per key head) are left to another kernel
 };
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// codes (unsigned) x digits (signed)
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_u8s8_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -68,59 +87,69 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// Two four-bit codes, at bits 4 * i and 16 + 4 * i of w, as the BF16 numbers 128 + code.
+// Four-bit codes of two tokens, at bits 0..3 and 16..19 of w (i = 0) or at bits 4..7 and 20..23 (i = 1), less the tokens'
+// zero points, as FP16: the mask-and-or gives 1024 + code (1024 + 16 * code), and what is subtracted is 1024 + zero
+// (64 + zero).
 template <int i>
-__device__ __forceinline__ uint32_t codes_pair(uint32_t w) {
-  return ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, uint32_t ones, uint32_t minus_low, uint32_t minus_high) {
+  uint32_t x;
+  if constexpr (i == 0) {
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(x) : "r"(w), "r"(ones));   // (w & mask) | ones, ones = 0x64006400
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(minus_low));
+  } else {
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(x) : "r"(w), "r"(ones));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x) : "r"(0x2c002c00u), "r"(minus_high));   // * 1/16
+  }
+  return x;
 }
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+__device__ __forceinline__ uint32_t lds32(const uint8_t* at) { return *reinterpret_cast<const uint32_t*>(at); }
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[1]) { w[0] = lds32(at); }
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[2]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(at);
+  w[0] = v.x; w[1] = v.y;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
+__device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[4]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(at);
+  w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
 }
-__device__ __forceinline__ void lds_words(uint32_t at, uint32_t (&w)[1]) { w[0] = lds32(at); }
-__device__ __forceinline__ void lds_words(uint32_t at, uint32_t (&w)[2]) {
-  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+// Sixteen bytes to shared memory past the registers and the L1; what is beyond `bytes` is filled with zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void lds_words(uint32_t at, uint32_t (&w)[4]) {
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
 // Number of keys the last row of a block of query rows sees, and the tiles they make (one at least: rows that see
 // nothing have to be written too).
-__device__ __forceinline__ int kv4_block_keys(const Kv4Sequence& s, int group, int rows_per_block, int block) {
-  const int last = min(s.rows * group, (block + 1) * rows_per_block) - 1;
-  return max(0, s.keys - s.rows + last / group + 1);
+__device__ __forceinline__ int kv4_block_keys(const Kv4Sequence& s, const Kv4Divisor& group, int rows_per_block, int block) {
+  const int last = min(s.rows * static_cast<int>(group.d), (block + 1) * rows_per_block) - 1;
+  return max(0, s.keys - s.rows + group.quotient(last) + 1);
 }
 __device__ __forceinline__ int kv4_block_tiles(int keys) { return max(1, (keys + kKv4Tile - 1) / kKv4Tile); }
 // Tiles of one key head of a sequence.
-__device__ __forceinline__ long long kv4_head_tiles(const Kv4Sequence& s, int group, int rows_per_block, int most_rows) {
-  const int rows = s.rows * group;
+__device__ __forceinline__ long long kv4_head_tiles(const Kv4Sequence& s, const Kv4Divisor& group, int rows_per_block, int most_rows) {
+  const int rows = s.rows * static_cast<int>(group.d);
   if (rows == 0 || rows > most_rows) return 0;
   long long tiles = 0;
+#pragma unroll 1
   for (int block = 0; block * rows_per_block < rows; ++block) tiles += kv4_block_tiles(kv4_block_keys(s, group, rows_per_block, block));
   return tiles;
 }
 
 // What a warp leaves of a sequence it shares with a neighbour.
 struct Kv4Piece {
-  int b, head, block, kind;       // kind: 0 none, 1 ends the sequence's tiles (in the workspace), 2 open at its end (in the ring)
+  int kind;                       // 0 none, 1 ends the sequence's tiles (in the workspace), 2 open at its end (in the ring)
   int starts;                     // it holds the first tile
-  long long first, tiles;         // place of the first tile among all, number of tiles
+  unsigned first, tiles;          // place of the first tile among all, number of tiles
+  int start, row, rows, head;     // first token row of the sequence, first query row of the block, its rows, key head
 };
 
 template <int kDim, int kQ>
@@ -131,173 +160,213 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   constexpr int kVWords = kDim / 64;                     // a lane's words of a value row
   constexpr int kLoad = kKWords > 4 ? 4 : kKWords;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ int4 infos[kWarps][kStages];
-  __shared__ long long prefix[kThreads + 1];
+  __shared__ long long scans[kThreads], warp_sums[kWarps];
   __shared__ Kv4Piece pieces[2 * kWarps];
   __shared__ Kv4Piece shared_units[2];                   // sequences shared with the CTA before [0] and behind [1]
-  __shared__ float inverse_sums[kRows];
-  __shared__ int abort_flag, comes_last[2];
+  __shared__ float piece_m[2 * kWarps][kRows], piece_l[2 * kWarps][kRows], group_m[2 * kWarps][kRows], group_l[2 * kWarps][kRows];
+  __shared__ float weights[2 * kWarps][kRows], inverse_sums[kRows];
+  __shared__ int comes_last[2];
   const Kv4AttendParams& p = params.a;
   const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32, g = lane / 4, c = lane % 4;
-  const int group = p.q_heads / p.kv_heads;
+  const int group = p.group.d;
 
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(&bars[warp][s]), 1);
-  }
-  if (thread == 0) abort_flag = 0;
   if (thread < 2 * kWarps) pieces[thread].kind = 0;
   if (thread < 2) shared_units[thread].kind = comes_last[thread] = 0;
-  fence_barrier_init();
   pdl_wait();
   pdl_launch_dependents();
 
   // ---- every tile's place: thread t sums the sequences of its share, then a scan over the threads
   const int share = (p.batch + kThreads - 1) / kThreads;
-  long long mine = 0;
+  long long scan = 0;
   for (int b = thread * share; b < min(p.batch, (thread + 1) * share); ++b)
-    mine += kv4_head_tiles(kv4_sequence(p, b), group, kRows, params.most_rows) * p.kv_heads;
-  long long scan = mine;
+    scan += kv4_head_tiles(kv4_sequence(p, b), p.group, kRows, params.most_rows) * p.kv_heads;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const long long other = __shfl_up_sync(0xffffffffu, scan, d);
     if (lane >= d) scan += other;
   }
-  __shared__ long long warp_sums[kWarps];
+  scans[thread] = scan;
   if (lane == 31) warp_sums[warp] = scan;
   __syncthreads();
-  long long before = 0;
-  for (int w = 0; w < warp; ++w) before += warp_sums[w];
-  prefix[thread + 1] = before + scan;
-  if (thread == 0) prefix[0] = 0;
-  __syncthreads();
-  const long long total = prefix[kThreads];
-  if (total == 0) return;
-  // as many CTAs as give every warp a few tiles: below that, joining costs more than the tiles
-  constexpr int kLeast = 2;
-  long long ctas = (total + kWarps * kLeast - 1) / (kWarps * kLeast);
-  if (ctas > gridDim.x) ctas = gridDim.x;
+  long long sums = lane < kWarps ? warp_sums[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < kWarps; d *= 2) {
+    const long long other = __shfl_up_sync(0xffffffffu, sums, d);
+    if (lane >= d) sums += other;
+  }
+  const long long all_tiles = __shfl_sync(0xffffffffu, sums, kWarps - 1);
+  if (all_tiles == 0) return;
+  if (all_tiles >> 31) {                                 // only overlapping sequences can come to that: refused
+    if (thread == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
+    return;
+  }
+  const unsigned total = static_cast<unsigned>(all_tiles);
+  // No more CTAs than get kLeast tiles each: below that, joining them costs more than the tiles.
+  constexpr unsigned kLeast = 4;
+  const unsigned ctas = min(gridDim.x, (total + kLeast - 1) / kLeast);
   if (blockIdx.x >= ctas) return;
-  const long long workers = ctas * kWarps;
-  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long range = worker * total / workers, range_end = (worker + 1) * total / workers;
-  const int count = static_cast<int>(range_end - range);
+  const unsigned per_cta = total / ctas, longer = total - per_cta * ctas;   // the first `longer` CTAs take one more
+  const unsigned cta_tiles = per_cta + (blockIdx.x < longer ? 1 : 0);
+  const unsigned cta_first = blockIdx.x * per_cta + min(blockIdx.x, longer);
+  const int per_warp = cta_tiles / kWarps, more = cta_tiles % kWarps;
+  const int count = per_warp + (warp < more ? 1 : 0);
+  const unsigned range = cta_first + warp * per_warp + min(warp, more);
 
   // ---- where this warp's range begins
   int b = 0, head = 0, block = 0, tile = 0, keys = 0, tiles = 0;
   Kv4Sequence seq{};
   if (count > 0) {
-    int low = 0, high = kThreads;                        // the thread whose share holds the first tile
-    while (high - low > 1) {
-      const int mid = (low + high) / 2;
-      if (prefix[mid] <= range) low = mid; else high = mid;
-    }
-    long long rest = range - prefix[low], per_head = 0;
-    for (b = low * share;; ++b) {
+    const int w = __popc(__ballot_sync(0xffffffffu, lane < kWarps && sums <= range));           // the warp, then the thread
+    const long long before = w ? __shfl_sync(0xffffffffu, sums, w - 1) : 0;
+    const long long within = scans[w * 32 + lane];
+    const int t = __popc(__ballot_sync(0xffffffffu, before + within <= range));                 // whose share holds the first tile
+    unsigned rest = range - static_cast<unsigned>(before) - (t ? static_cast<unsigned>(__shfl_sync(0xffffffffu, within, t - 1)) : 0);
+    unsigned per_head = 0;
+    for (b = (w * 32 + t) * share;; ++b) {
       seq = kv4_sequence(p, b);
-      per_head = kv4_head_tiles(seq, group, kRows, params.most_rows);
+      per_head = static_cast<unsigned>(kv4_head_tiles(seq, p.group, kRows, params.most_rows));
       if (rest < per_head * p.kv_heads) break;
       rest -= per_head * p.kv_heads;
     }
-    head = static_cast<int>(rest / per_head);
+    head = rest / per_head;
     rest -= head * per_head;
     for (block = 0;; ++block) {
-      keys = kv4_block_keys(seq, group, kRows, block);
+      keys = kv4_block_keys(seq, p.group, kRows, block);
       tiles = kv4_block_tiles(keys);
-      if (rest < tiles) break;
+      if (rest < static_cast<unsigned>(tiles)) break;
       rest -= tiles;
     }
-    tile = static_cast<int>(rest);
+    tile = rest;
   }
 
-  // ---- the loader's side of the ring: tiles of the range in order, one ahead of what it has issued (page numbers are
-  // fetched one tile early)
+  // ---- the loader's side of the ring: the tiles of the range in order, copied by the lanes in pieces of 16 bytes (a tile
+  // touches one page, or two of 16 tokens); the lanes hold the next 32 page numbers of the sequence
   const int page = 1 << p.page_shift;
-  const int64_t block_bytes = kv4_block_bytes(page, kDim);
+  const int64_t block_bytes = kv4_block_bytes(page, kDim), page_bytes = block_bytes * kKv4Side * p.kv_heads;
   const uint32_t ring_base = smem_u32(ring) + warp * kStages * Cfg::kStageBytes;
-  const int part_rows = page < kKv4Tile ? page : kKv4Tile, parts = kKv4Tile / part_rows;
-  const int part = lane >> 2, piece_of = lane & 3;       // lanes 0..4 * parts - 1 issue a copy each
-  int page_id = -1;
-  auto fetch_page = [&]() {
-    const int token = tile * kKv4Tile + part * part_rows;
-    page_id = -1;
-    if (part < parts && token < keys) page_id = p.block_table[static_cast<int64_t>(b) * p.width + (token >> p.page_shift)];
+  const bool two_parts = page < kKv4Tile;
+  constexpr int kRowPieces = kDim / 32;                  // 16-byte pieces of a code row
+  const int lane_row = lane / kRowPieces;                // the lane's row among those one copy instruction covers
+  const uint32_t lane_code = ring_base + 16 * lane;
+  const uint8_t* head_src = nullptr;
+  int window = -1, window_first = 0;
+  auto load_window = [&]() {
+    window_first = tile * kKv4Tile >> p.page_shift;      // even when a tile touches two pages
+    const int index = window_first + lane;
+    window = static_cast<int64_t>(index) << p.page_shift < keys ? p.block_table[static_cast<int64_t>(b) * p.width + index] : -1;
+  };
+  auto begin_unit = [&]() {
+    head_src = p.cache + head * block_bytes;
+    load_window();
   };
   auto issue = [&](int stage) {
-    const int token = tile * kKv4Tile + part * part_rows;
-    const int rows = part < parts ? min(part_rows, max(0, keys - token)) : 0;
-    const bool wanted = rows > 0, good = wanted && page_id >= 0 && page_id < p.pages;
-    if (wanted && !good && piece_of == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
-    const int copied = good ? (rows + 3) & ~3 : 0;       // rows in fours: 16-byte multiples
-    const uint32_t bytes = piece_of & 1 ? copied * 4 : copied * (kDim / 2);
-    const uint32_t goods = __ballot_sync(0xffffffffu, good);
-    const uint32_t sum = __reduce_add_sync(0xffffffffu, bytes);
-    const uint32_t bar = smem_u32(&bars[warp][stage]);
-    if (lane == 0) {
-      const int flags = (goods & 1u ? 1 : 0) | (goods & 16u ? 2 : 0) | (tile == tiles - 1 ? 4 : 0);
-      infos[warp][stage] = make_int4(b, head, block, (tile << 3) | flags);
-      mbar_arrive_expect_tx(bar, sum);
+    const int token = tile * kKv4Tile;
+    const int rows = min(kKv4Tile, keys - token);        // none or fewer: rows that see nothing
+    int index = (token >> p.page_shift) - window_first;
+    if (index >= 32) {
+      load_window();
+      index = 0;
     }
-    __syncwarp();
-    if (bytes) {
-      const uint8_t* src = p.cache + ((static_cast<int64_t>(page_id) * kKv4Side + (piece_of >> 1)) * p.kv_heads + head) * block_bytes;
-      const int row = token & (page - 1);
-      src += piece_of & 1 ? page * (kDim / 2) + 4 * row : row * (kDim / 2);
-      const uint32_t dst = ring_base + stage * Cfg::kStageBytes + (piece_of >> 1) * (Cfg::kCodeBytes + Cfg::kPairBytes) +
-                           (piece_of & 1 ? Cfg::kCodeBytes + part * part_rows * 4 : part * part_rows * (kDim / 2));
-      bulk_load(dst, src, bytes, bar);
+    const int page0 = __shfl_sync(0xffffffffu, window, index), page1 = __shfl_sync(0xffffffffu, window, index + (two_parts ? 1 : 0));
+    bool good0 = static_cast<unsigned>(page0) < static_cast<unsigned>(p.pages);
+    bool good1 = static_cast<unsigned>(page1) < static_cast<unsigned>(p.pages);
+    if (((rows > 0 && !good0) || (rows > 16 && !good1)) && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
+    good0 = good0 && rows > 0;
+    good1 = good1 && rows > 16;
+    if (lane == 0) infos[warp][stage] = make_int4(b, head, block, (tile << 3) | (good0 ? 1 : 0) | (good1 ? 2 : 0) | (tile == tiles - 1 ? 4 : 0));
+    const int row = token & (page - 1);
+    const uint8_t* src0 = good0 ? head_src + page0 * page_bytes : p.cache;
+    const uint8_t* src1 = two_parts ? (good1 ? head_src + page1 * page_bytes : p.cache) : src0 + 16 * (kDim / 2);
+    const int64_t value_offset = p.kv_heads * block_bytes;
+    const uint8_t* code0 = src0 + row * (kDim / 2) + 16 * lane;
+    const uint8_t* code1 = src1 + (two_parts ? 0 : row * (kDim / 2)) + 16 * lane;
+    const uint32_t dst = lane_code + stage * Cfg::kStageBytes;
+    constexpr int kCopies = kRowPieces / 2;              // copy instructions for 16 rows of codes
+    // the pairs: lanes 0..7 the keys', 8..15 the values', four tokens each
+    const int pair_token = 4 * (lane & 7);
+    const bool pair_second = pair_token >= 16;
+    const uint8_t* pair_src = (two_parts && pair_second ? src1 - 64 : src0 + 4 * row) + page * (kDim / 2) + 4 * pair_token +
+                              (lane & 8 ? value_offset : 0);
+    const uint32_t pair_dst = ring_base + stage * Cfg::kStageBytes + Cfg::kCodeBytes + 4 * pair_token +
+                              (lane & 8 ? Cfg::kCodeBytes + Cfg::kPairBytes : 0);
+    if (rows == kKv4Tile && good0 && good1) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        copy16(dst + 512 * i, code0 + 512 * i, 16);
+        copy16(dst + 512 * (kCopies + i), code1 + 512 * i, 16);
+        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * i, code0 + value_offset + 512 * i, 16);
+        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * (kCopies + i), code1 + value_offset + 512 * i, 16);
+      }
+      if (lane < 16) copy16(pair_dst, pair_src, 16);
+    } else {
+      // rows behind the last key or on a page that cannot be followed are filled with zeros: scale 0, zero point 0
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = lane_row + i * (32 / kRowPieces);
+        const int bytes0 = good0 && r < rows ? 16 : 0, bytes1 = good1 && r + 16 < rows ? 16 : 0;
+        copy16(dst + 512 * i, bytes0 ? code0 + 512 * i : p.cache, bytes0);
+        copy16(dst + 512 * (kCopies + i), bytes1 ? code1 + 512 * i : p.cache, bytes1);
+        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * i, bytes0 ? code0 + value_offset + 512 * i : p.cache, bytes0);
+        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * (kCopies + i), bytes1 ? code1 + value_offset + 512 * i : p.cache, bytes1);
+      }
+      if (lane < 16) {
+        const int bytes = (pair_second ? good1 : good0) ? 4 * max(0, min(4, rows - pair_token)) : 0;
+        copy16(pair_dst, bytes ? pair_src : p.cache, bytes);
+      }
     }
-    // the next tile
-    if (++tile == tiles) {
+    if (++tile == tiles) {                               // the next block of rows, head or sequence
       tile = 0;
       if (++block * kRows >= seq.rows * group) {
         block = 0;
         if (++head == p.kv_heads) {
           head = 0;
           do {
-            ++b;
-            if (b < p.batch) seq = kv4_sequence(p, b);
+            if (++b < p.batch) seq = kv4_sequence(p, b);
           } while (b < p.batch && (seq.rows == 0 || seq.rows * group > params.most_rows));
         }
       }
       if (b < p.batch) {
-        keys = kv4_block_keys(seq, group, kRows, block);
+        keys = kv4_block_keys(seq, p.group, kRows, block);
         tiles = kv4_block_tiles(keys);
+        begin_unit();
       }
     }
-    if (b < p.batch) fetch_page();
+    __syncwarp();                                        // the tile's description is there for every lane
   };
-  int issued = 0;
-  if (count > 0) fetch_page();
-  for (; issued < min(count, kStages); ++issued) issue(issued);
-
+  if (count > 0) begin_unit();
   // ---- the consumer's side
   float o[4 * kVWords][kQ][4];
-  float m[kQ][2], sum[kQ][2], qsum[kQ][2];
+  float m[kQ][2], sum[kQ][2], qscale[kQ][2];
+  int qsum[kQ][2];
+  float most_scale = 0.f, value_unit = 1.f;              // power of two above the values' scales so far; 128 / it
   int limit[kQ][2];
-  uint32_t q[2 * kKWords][kQ][2];
-  int cur_b = 0, cur_head = 0, cur_block = 0, cur_tile = 0, cur_rows = 0, cur_start = 0, cur_keys = 0, unit_first_tile = 0;
+  uint32_t q[kKWords][kQ][4];                            // high digits (even, odd components of a word), low digits
+  int cur_b = 0, cur_head = 0, cur_block = 0, cur_tile = 0, cur_rows = 0, cur_start = 0, cur_keys = 0, first_tile = 0;
   int least = 0;
-  bool fresh = true, open = false;
+  bool fresh = true;
   const int turned = g ^ ((g >> 1) & 1);                 // which token of eight a row of S^T holds: spreads the reads over the banks
-  const int t_even = 2 * c ^ (c & 1), t_odd = (2 * c + 1) ^ (c & 1);
+  uint32_t ones;                                         // kept in a register: an immediate would cost a second instruction
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(ones));
+  const int t_even = (2 * c) ^ (c & 1), t_odd = (2 * c + 1) ^ (c & 1);
 
-  // Writes this warp's maximum, sum and output of every row: [maximum][sum][output].
-  auto write_piece = [&](float* dst) {
+  // Leaves this warp's maximum, sum (in piece_m, piece_l) and output of every row.
+  auto write_piece = [&](int piece, float* dst) {
+    const float unit = 1.f / value_unit;                 // a power of two
 #pragma unroll
     for (int n = 0; n < kQ; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = 8 * n + 2 * c + e;
         if (g == 0) {
-          dst[row] = m[n][e];
-          dst[kRows + row] = sum[n][e];
+          piece_m[piece][row] = m[n][e];
+          piece_l[piece][row] = sum[n][e];
         }
 #pragma unroll
         for (int k = 0; k < kVWords; ++k) {
-          float4* to = reinterpret_cast<float4*>(dst + 2 * kRows + row * kDim + 8 * (kVWords * g + k));
-          to[0] = make_float4(o[4 * k][n][e], o[4 * k + 1][n][e], o[4 * k + 2][n][e], o[4 * k + 3][n][e]);
-          to[1] = make_float4(o[4 * k][n][2 + e], o[4 * k + 1][n][2 + e], o[4 * k + 2][n][2 + e], o[4 * k + 3][n][2 + e]);
+          float4* to = reinterpret_cast<float4*>(dst + row * kDim + 8 * (kVWords * g + k));
+          to[0] = make_float4(o[4 * k][n][e] * unit, o[4 * k + 1][n][e] * unit, o[4 * k + 2][n][e] * unit, o[4 * k + 3][n][e] * unit);
+          to[1] = make_float4(o[4 * k][n][2 + e] * unit, o[4 * k + 1][n][2 + e] * unit, o[4 * k + 2][n][2 + e] * unit, o[4 * k + 3][n][2 + e] * unit);
         }
       }
   };
@@ -311,229 +380,281 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         sum[n][e] += __shfl_xor_sync(0xffffffffu, sum[n][e], 16);
       }
   };
-  float* const head_slot = params.slots + (2ll * gridDim.x + worker) * Cfg::kPieceFloats;
-
-  for (int it = 0; it < count; ++it) {
-    const int stage = it % kStages;
-    if (!mbar_wait(smem_u32(&bars[warp][stage]), (it / kStages) & 1, &abort_flag)) {
-      int gave_up = 0;                                   // the copies in flight still write here: wait for them, with the same limit
-      for (int k = it; k < issued && !gave_up; ++k) mbar_wait(smem_u32(&bars[warp][k % kStages]), (k / kStages) & 1, &gave_up);
-      break;
-    }
-    const int4 info = infos[warp][stage];
-    cur_tile = info.w >> 3;
-    if (fresh) {
-      fresh = false;
-      open = true;
-      cur_b = info.x; cur_head = info.y; cur_block = info.z;
-      unit_first_tile = cur_tile;
-      const Kv4Sequence s = kv4_sequence(p, cur_b);
-      cur_rows = s.rows * group;
-      cur_start = s.start;
-      cur_keys = kv4_block_keys(s, group, kRows, cur_block);
-      least = 0x7fffffff;
+  // Queries of a block of rows: lane (g, c) holds row g's words c as digits, in the order of a word's two masks.
+  auto load_queries = [&]() {
+    const Kv4Sequence s = kv4_sequence(p, cur_b);
+    cur_rows = s.rows * group;
+    cur_start = s.start;
+    cur_keys = kv4_block_keys(s, p.group, kRows, cur_block);
+    least = 0x7fffffff;
+    most_scale = 0.f;
+    value_unit = 1.f;
 #pragma unroll
-      for (int n = 0; n < kQ; ++n) {
-        // queries: lane (g, c) holds row g's words c, in the order in which the keys' codes come out of a word
-        const int row = cur_block * kRows + 8 * n + g;
-        float part_sum = 0.f;
+    for (int n = 0; n < kQ; ++n) {
+      const int row = cur_block * kRows + 8 * n + g, row_token = p.group.quotient(row);
+      const uint16_t* src = p.q + (cur_start + row_token) * p.q_stride + static_cast<int64_t>(cur_head * group + row - row_token * group) * kDim;
+      uint4 w[kKWords];
+      float most = 0.f;
 #pragma unroll
-        for (int k = 0; k < kKWords; ++k) {
-          const int word = kLoad * c + (k % kLoad) + (k / kLoad) * 4 * kLoad;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (row < cur_rows)
-            w = *reinterpret_cast<const uint4*>(p.q + (cur_start + row / group) * p.q_stride +
-                                                static_cast<int64_t>(cur_head * group + row % group) * kDim + 8 * word);
-          float x[8];
-          unpack8(w, x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) part_sum += x[j];
-          q[2 * k][n][0] = __byte_perm(w.x, w.z, 0x5410);
-          q[2 * k][n][1] = __byte_perm(w.x, w.z, 0x7632);
-          q[2 * k + 1][n][0] = __byte_perm(w.y, w.w, 0x5410);
-          q[2 * k + 1][n][1] = __byte_perm(w.y, w.w, 0x7632);
-        }
-        part_sum += __shfl_xor_sync(0xffffffffu, part_sum, 1);
-        part_sum += __shfl_xor_sync(0xffffffffu, part_sum, 2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int column = cur_block * kRows + 8 * n + 2 * c + e;
-          qsum[n][e] = __shfl_sync(0xffffffffu, part_sum, 8 * c + 4 * e);
-          limit[n][e] = column < cur_rows ? max(0, s.keys - s.rows + column / group + 1) : 0x7fffffff;
-          least = min(least, limit[n][e]);
-          m[n][e] = -INFINITY;
-          sum[n][e] = 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 4 * kVWords; ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[k][n][j] = 0.f;
-      }
-      least = __reduce_min_sync(0xffffffffu, least);
-    }
-    const uint32_t keys_at = ring_base + stage * Cfg::kStageBytes, values_at = keys_at + Cfg::kCodeBytes + Cfg::kPairBytes;
-    const int first = cur_tile * kKv4Tile;
-    // a tile with tokens behind the last one some row sees, or on a page that could not be followed
-    const bool whole = first + kKv4Tile <= least && (info.w & 3) == (parts == 2 ? 3 : 1);
-    auto usable = [&](int t) { return (info.w >> (parts == 2 ? t >> 4 : 0)) & 1; };
-
-    // S^T = K Q^T
-    float s[2][kQ][4];
-    float kscale[2][2], kzero[2][2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int n = 0; n < kQ; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[mt][n][j] = 0.f;
-      const int t0 = 16 * mt + turned;
-#pragma unroll
-      for (int j = 0; j < kKWords; j += kLoad) {
-        uint32_t wa[kLoad], wb[kLoad];
-        const uint32_t at = keys_at + t0 * (kDim / 2) + 4 * (kLoad * c + j * 4);
-        lds_words(at, wa);
-        lds_words(at + 8 * (kDim / 2), wb);
-#pragma unroll
-        for (int k = 0; k < kLoad; ++k) {
-#pragma unroll
-          for (int n = 0; n < kQ; ++n)
-            mma_bf16(s[mt][n], codes_pair<0>(wa[k]), codes_pair<0>(wb[k]), codes_pair<1>(wa[k]), codes_pair<1>(wb[k]),
-                     q[2 * (j + k)][n][0], q[2 * (j + k)][n][1]);
-#pragma unroll
-          for (int n = 0; n < kQ; ++n)
-            mma_bf16(s[mt][n], codes_pair<2>(wa[k]), codes_pair<2>(wb[k]), codes_pair<3>(wa[k]), codes_pair<3>(wb[k]),
-                     q[2 * (j + k) + 1][n][0], q[2 * (j + k) + 1][n][1]);
-        }
+      for (int k = 0; k < kKWords; ++k) {
+        const int word = kLoad * c + (k % kLoad) + (k / kLoad) * 4 * kLoad;
+        w[k] = make_uint4(0, 0, 0, 0);
+        if (row < cur_rows)
+          w[k] = *reinterpret_cast<const uint4*>(src + 8 * word);
       }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t pair = lds32(keys_at + Cfg::kCodeBytes + 4 * (t0 + 8 * r));
-        kscale[mt][r] = bf16_lo(pair) * p.scale_log2;
-        kzero[mt][r] = -128.f - bf16_hi(pair);
+      for (int k = 0; k < kKWords; ++k) {
+        float x[8];
+        unpack8(w[k], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = max_abs_keep_nan(most, x[j]);
       }
-    }
-    float top[kQ][2];
+      most = fabsf(most);
+      most = max_abs_keep_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fabsf(max_abs_keep_nan(most, __shfl_xor_sync(0xffffffffu, most, 2)));
+      const float scale = most > 0.f ? 32639.f / most : 0.f;             // 127 * 256 + 127
+      // a row with a NaN or an infinity is NaN as a whole
+      const float unit = most < INFINITY ? most * (1.f / 32639.f) * p.scale_log2 : __int_as_float(0x7fffffff);
+      int digits_sum = 0;
 #pragma unroll
-    for (int n = 0; n < kQ; ++n) top[n][0] = top[n][1] = -INFINITY;
+      for (int k = 0; k < kKWords; ++k) {
+        float x[8];
+        unpack8(w[k], x);
+        // x * scale rounded to an integer by adding 1.5 * 2^23: its low byte is the low digit; with 128 more, its second
+        // byte is the high one
+        uint32_t low[8], high[8];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int n = 0; n < kQ; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = fmaf(kzero[mt][j / 2], qsum[n][j % 2], s[mt][n][j]) * kscale[mt][j / 2];
-          if (!whole) {
-            const int t = 16 * mt + turned + 8 * (j / 2);
-            if (first + t >= limit[n][j % 2] || !usable(t)) x = -INFINITY;
-          }
-          s[mt][n][j] = x;
-          top[n][j % 2] = fmaxf(top[n][j % 2], x);
+        for (int j = 0; j < 8; ++j) {
+          low[j] = __float_as_uint(fmaf(x[j], scale, 12582912.f));
+          high[j] = __float_as_uint(fmaf(x[j], scale, 12582912.f + 128.f));
         }
-    bool grows = false;
 #pragma unroll
-    for (int n = 0; n < kQ; ++n)
+        for (int odd = 0; odd < 2; ++odd) {
+          q[k][n][odd] = __byte_perm(__byte_perm(high[odd], high[2 + odd], 0x0051), __byte_perm(high[4 + odd], high[6 + odd], 0x0051), 0x5410);
+          q[k][n][2 + odd] = __byte_perm(__byte_perm(low[odd], low[2 + odd], 0x0040), __byte_perm(low[4 + odd], low[6 + odd], 0x0040), 0x5410);
+          digits_sum += 256 * __dp4a(static_cast<int>(q[k][n][odd]), 0x01010101, 0) + __dp4a(static_cast<int>(q[k][n][2 + odd]), 0x01010101, 0);
+        }
+      }
+      digits_sum += __shfl_xor_sync(0xffffffffu, digits_sum, 1);
+      digits_sum += __shfl_xor_sync(0xffffffffu, digits_sum, 2);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
-        top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
-        top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16));
-        grows |= top[n][e] > m[n][e] + 8.f;
+        const int column = cur_block * kRows + 8 * n + 2 * c + e;
+        qsum[n][e] = __shfl_sync(0xffffffffu, digits_sum, 8 * c + 4 * e);
+        qscale[n][e] = __shfl_sync(0xffffffffu, unit, 8 * c + 4 * e);
+        limit[n][e] = column < cur_rows ? max(0, s.keys - s.rows + p.group.quotient(column) + 1) : 0x7fffffff;
+        least = min(least, limit[n][e]);
+        m[n][e] = -INFINITY;
+        sum[n][e] = 0.f;
       }
-    // The maximum follows only when it has grown by more than 2^8: weights up to 256 cost nothing in FP32 or BF16, and
-    // the output is rarely scaled again.
-    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int k = 0; k < 4 * kVWords; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[k][n][j] = 0.f;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+  };
+  float* const head_slot = params.slots + (2ll * gridDim.x + static_cast<long long>(blockIdx.x) * kWarps + warp) * Cfg::kPieceFloats;
+
+  int stage = 0;
+  // The first kStages rounds only fill the ring. Every round closes one group of copies, empty ones too: the waits count groups.
+#pragma unroll 1
+  for (int it = -kStages; it < count; ++it) {
+    int4 info = make_int4(0, 0, 0, 0);
+    if (it >= 0) {
+      info = infos[warp][stage];
+      cur_tile = info.w >> 3;
+      if (fresh) {
+        fresh = false;
+        cur_b = info.x; cur_head = info.y; cur_block = info.z;
+        first_tile = cur_tile;
+        load_queries();
+      }
+      copies_wait<kStages - 1>();
+      __syncwarp();
+      const uint8_t* keys_at = ring + (warp * kStages + stage) * Cfg::kStageBytes;
+      const uint8_t* values_at = keys_at + Cfg::kCodeBytes + Cfg::kPairBytes;
+      const int first = cur_tile * kKv4Tile;
+      // not whole: a tile with tokens behind the last one that some row sees, or on a page that could not be followed
+      const bool whole = first + kKv4Tile <= least && (info.w & 3) == 3;
+      auto usable = [&](int t) { return (info.w >> (t >> 4)) & 1; };
+
+      // S^T = K Q^T, in units of key scale * query unit
+      float s[2][kQ][4], top[kQ][2], vscale[2][2];
+#pragma unroll
+      for (int n = 0; n < kQ; ++n) top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        int high[kQ][4], low[kQ][4];
+        const int t0 = 16 * mt + turned;
+#pragma unroll
+        for (int j = 0; j < kKWords; j += kLoad) {
+          uint32_t wa[kLoad], wb[kLoad];
+          const uint8_t* at = keys_at + t0 * (kDim / 2) + 4 * (kLoad * c + j * 4);
+          lds_words(at, wa);
+          lds_words(at + 8 * (kDim / 2), wb);
+#pragma unroll
+          for (int k = 0; k < kLoad; ++k) {
+            const uint32_t a0 = wa[k] & 0x0f0f0f0fu, a1 = wb[k] & 0x0f0f0f0fu, a2 = (wa[k] >> 4) & 0x0f0f0f0fu, a3 = (wb[k] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+            for (int n = 0; n < kQ; ++n) {
+              const uint32_t(&d)[4] = q[j + k][n];
+              if (j + k == 0) {
+                mma_u8s8_first(high[n], a0, a1, a2, a3, d[0], d[1]);
+                mma_u8s8_first(low[n], a0, a1, a2, a3, d[2], d[3]);
+              } else {
+                mma_u8s8(high[n], a0, a1, a2, a3, d[0], d[1]);
+                mma_u8s8(low[n], a0, a1, a2, a3, d[2], d[3]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int t = t0 + 8 * r;
+          const uint32_t key_pair = lds32(keys_at + Cfg::kCodeBytes + 4 * t);
+          vscale[mt][r] = bf16_lo(lds32(values_at + Cfg::kCodeBytes + 4 * t));
+          const float kscale = bf16_lo(key_pair);
+          const int zero = __float2int_rn(bf16_hi(key_pair));
+#pragma unroll
+          for (int n = 0; n < kQ; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // below 2^28: exact
+              s[mt][n][2 * r + e] = static_cast<float>(high[n][2 * r + e] * 256 + low[n][2 * r + e] - zero * qsum[n][e]) * kscale;
+            }
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int n = 0; n < kQ; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int t = 16 * mt + turned + 8 * (j / 2);
+              if (first + t >= limit[n][j % 2] || !usable(t)) s[mt][n][j] = -INFINITY;
+            }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int n = 0; n < kQ; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[n][j % 2] = fmaxf(top[n][j % 2], s[mt][n][j]);
+      const float tile_scale = __uint_as_float(__reduce_max_sync(
+          0xffffffffu, __float_as_uint(fmaxf(fmaxf(vscale[0][0], vscale[0][1]), fmaxf(vscale[1][0], vscale[1][1])))));
+      bool grows = tile_scale > most_scale;
 #pragma unroll
       for (int n = 0; n < kQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float next = fmaxf(m[n][e], top[n][e]);
-          const float keep = next == -INFINITY ? 1.f : fast_exp2(m[n][e] - next);
-          m[n][e] = next;
-          sum[n][e] *= keep;
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16)) * qscale[n][e];
+          grows |= top[n][e] > m[n][e] + 8.f;
+        }
+      // The maximum follows only when it has grown by more than 2^8 (weights up to 256 fit), so that the output is rarely
+      // scaled again.
+      if (__any_sync(0xffffffffu, grows)) {
+        float turn = 1.f;
+        if (tile_scale > most_scale) {
+          most_scale = __uint_as_float((__float_as_uint(tile_scale) + 0x007fffffu) & 0xff800000u);
+          const float next = 128.f / most_scale;
+          turn = next / value_unit;
+          value_unit = next;
+        }
 #pragma unroll
-          for (int k = 0; k < 4 * kVWords; ++k) {
-            o[k][n][e] *= keep;
-            o[k][n][2 + e] *= keep;
+        for (int n = 0; n < kQ; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float next = fmaxf(m[n][e], top[n][e]);
+            float keep = next == -INFINITY ? 1.f : fast_exp2(m[n][e] - next);
+            m[n][e] = next;
+            sum[n][e] *= keep;
+            keep *= turn;
+#pragma unroll
+            for (int k = 0; k < 4 * kVWords; ++k) {
+              o[k][n][e] *= keep;
+              o[k][n][2 + e] *= keep;
+            }
+          }
+      }
+      // weights, times the values' scales, transposed into the second product's operand
+      uint32_t w[2][kQ][2];
+      float base[kQ][2];
+#pragma unroll
+      for (int n = 0; n < kQ; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) base[n][e] = m[n][e] == -INFINITY ? 0.f : -m[n][e];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const float scale[2] = {vscale[mt][0] * value_unit, vscale[mt][1] * value_unit};
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) {
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float weight = fast_exp2(fmaf(s[mt][n][j], qscale[n][j % 2], base[n][j % 2]));
+            sum[n][j % 2] += weight;
+            x[j] = weight * scale[j / 2];
+          }
+          w[mt][n][0] = transpose8x8(pack_f16(x[0], x[1]));
+          w[mt][n][1] = transpose8x8(pack_f16(x[2], x[3]));
+        }
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t minus_low[2], minus_high[2], v[4][kVWords];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int ta = 16 * mt + 8 * r + t_even, tb = 16 * mt + 8 * r + t_odd;
+          const uint32_t pa = lds32(values_at + Cfg::kCodeBytes + 4 * ta), pb = lds32(values_at + Cfg::kCodeBytes + 4 * tb);
+          // 128 + zero as BF16 has the zero point in its low bits, which then make -(1024 + zero) as FP16
+          uint32_t zeros = __byte_perm(pa, pb, 0x7632);
+          asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(zeros) : "r"(0x43004300u));
+          minus_low[r] = (zeros & 0x000f000fu) | 0xe400e400u;
+          asm("add.rn.f16x2 %0, %1, %2;" : "=r"(minus_high[r]) : "r"(minus_low[r]), "r"(0x63806380u));   // + 960
+          lds_words(values_at + ta * (kDim / 2) + 4 * kVWords * g, v[2 * r]);
+          lds_words(values_at + tb * (kDim / 2) + 4 * kVWords * g, v[2 * r + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < kVWords; ++k) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {           // components 0, 1 (4, 5), then 2, 3 (6, 7) of the word
+            const uint32_t lo0 = __byte_perm(v[0][k], v[1][k], half ? 0x0501 : 0x0400), hi0 = __byte_perm(v[0][k], v[1][k], half ? 0x0703 : 0x0602);
+            const uint32_t lo1 = __byte_perm(v[2][k], v[3][k], half ? 0x0501 : 0x0400), hi1 = __byte_perm(v[2][k], v[3][k], half ? 0x0703 : 0x0602);
+            const uint32_t a0 = code_pair<0>(lo0, ones, minus_low[0], minus_high[0]), a1 = code_pair<0>(hi0, ones, minus_low[0], minus_high[0]);
+            const uint32_t a2 = code_pair<0>(lo1, ones, minus_low[1], minus_high[1]), a3 = code_pair<0>(hi1, ones, minus_low[1], minus_high[1]);
+            const uint32_t b0 = code_pair<1>(lo0, ones, minus_low[0], minus_high[0]), b1 = code_pair<1>(hi0, ones, minus_low[0], minus_high[0]);
+            const uint32_t b2 = code_pair<1>(lo1, ones, minus_low[1], minus_high[1]), b3 = code_pair<1>(hi1, ones, minus_low[1], minus_high[1]);
+#pragma unroll
+            for (int n = 0; n < kQ; ++n) {
+              mma_f16(o[4 * k + 2 * half][n], a0, a1, a2, a3, w[mt][n][0], w[mt][n][1]);
+              mma_f16(o[4 * k + 2 * half + 1][n], b0, b1, b2, b3, w[mt][n][0], w[mt][n][1]);
+            }
           }
         }
-    }
-    // weights, times the values' scales, transposed into the second product's operand
-    uint32_t w[2][kQ][2];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      float vscale[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int t = 16 * mt + turned + 8 * r;
-        uint32_t pair = lds32(values_at + Cfg::kCodeBytes + 4 * t);
-        if (!whole && (first + t >= cur_keys || !usable(t))) pair = 0;
-        vscale[r] = bf16_lo(pair);
       }
-#pragma unroll
-      for (int n = 0; n < kQ; ++n) {
-        float x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float base = m[n][j % 2] == -INFINITY ? 0.f : m[n][j % 2];
-          const float weight = fast_exp2(s[mt][n][j] - base);
-          sum[n][j % 2] += weight;
-          x[j] = weight * vscale[j / 2];
-        }
-        w[mt][n][0] = transpose8x8(pack2(x[0], x[1]));
-        w[mt][n][1] = transpose8x8(pack2(x[2], x[3]));
-      }
+      __syncwarp();                                      // every lane has read the stage
     }
-    // O^T += V^T P^T
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      uint32_t zero[2];
-      uint32_t v[4][kVWords];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int ta = 16 * mt + 8 * r + t_even, tb = 16 * mt + 8 * r + t_odd;
-        uint32_t pa = lds32(values_at + Cfg::kCodeBytes + 4 * ta), pb = lds32(values_at + Cfg::kCodeBytes + 4 * tb);
-        if (!whole) {
-          if (first + ta >= cur_keys || !usable(ta)) pa = 0;
-          if (first + tb >= cur_keys || !usable(tb)) pb = 0;
-        }
-        zero[r] = add_bf16x2(__byte_perm(pa, pb, 0x7632), 0x43004300u);
-        lds_words(values_at + ta * (kDim / 2) + 4 * kVWords * g, v[2 * r]);
-        lds_words(values_at + tb * (kDim / 2) + 4 * kVWords * g, v[2 * r + 1]);
-      }
-#pragma unroll
-      for (int k = 0; k < kVWords; ++k) {
-        const uint32_t lo0 = __byte_perm(v[0][k], v[1][k], 0x5410), hi0 = __byte_perm(v[0][k], v[1][k], 0x7632);
-        const uint32_t lo1 = __byte_perm(v[2][k], v[3][k], 0x5410), hi1 = __byte_perm(v[2][k], v[3][k], 0x7632);
-        auto step = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-          a0 = sub_bf16x2(a0, zero[0]);
-          a1 = sub_bf16x2(a1, zero[0]);
-          a2 = sub_bf16x2(a2, zero[1]);
-          a3 = sub_bf16x2(a3, zero[1]);
-#pragma unroll
-          for (int n = 0; n < kQ; ++n) mma_bf16(o[4 * k + i][n], a0, a1, a2, a3, w[mt][n][0], w[mt][n][1]);
-        };
-        step(0, codes_pair<0>(lo0), codes_pair<0>(hi0), codes_pair<0>(lo1), codes_pair<0>(hi1));
-        step(1, codes_pair<1>(lo0), codes_pair<1>(hi0), codes_pair<1>(lo1), codes_pair<1>(hi1));
-        step(2, codes_pair<2>(lo0), codes_pair<2>(hi0), codes_pair<2>(lo1), codes_pair<2>(hi1));
-        step(3, codes_pair<3>(lo0), codes_pair<3>(hi0), codes_pair<3>(lo1), codes_pair<3>(hi1));
-      }
-    }
-    __syncwarp();                                        // every lane has read the stage
-    if (issued < count) {
-      issue(stage);
-      ++issued;
-    }
+    if (it + kStages < count) issue(stage);
+    copies_commit();
+    if (++stage == kStages) stage = 0;
     if (info.w & 4) {                                    // the last tile of these rows
       add_sums();
-      if (unit_first_tile == 0) {
+      if (first_tile == 0) {
+        const float unit = 1.f / value_unit;
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int row = cur_block * kRows + 8 * n + 2 * c + e;
             if (row >= cur_rows) continue;
-            const float inverse = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
-            uint16_t* dst = p.out + (static_cast<int64_t>(cur_start + row / group) * p.q_heads + cur_head * group + row % group) * kDim;
+            const float inverse = sum[n][e] == 0.f ? 0.f : unit / sum[n][e];
+            const int row_token = p.group.quotient(row);
+            uint16_t* dst = p.out + (static_cast<int64_t>(cur_start + row_token) * p.q_heads + cur_head * group + row - row_token * group) * kDim;
 #pragma unroll
             for (int k = 0; k < kVWords; ++k) {
               float x[8];
@@ -546,78 +667,100 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
             }
           }
       } else {
-        write_piece(head_slot);
-        if (lane == 0) {
-          // only the first sequence of a range can have begun before it
-          pieces[2 * warp] = Kv4Piece{cur_b, cur_head, cur_block, 1, 0, range + it - cur_tile, cur_tile + 1};
-        }
+        write_piece(2 * warp, head_slot);                // only the first sequence of a range can have begun before it
+        if (lane == 0)
+          pieces[2 * warp] = Kv4Piece{1, 0, range + it - cur_tile, cur_tile + 1u, cur_start, cur_block * kRows,
+                                      min(kRows, cur_rows - cur_block * kRows), cur_head};
       }
       fresh = true;
-      open = false;
     }
   }
-  if (open) {                                            // the range ends inside a sequence: kept in the ring, which is idle now
+  if (!fresh) {                                          // the range ends inside a sequence: kept in the ring, which is idle now
     add_sums();
-    write_piece(reinterpret_cast<float*>(ring + warp * kStages * Cfg::kStageBytes));
-    if (lane == 0) {
-      const Kv4Sequence s = kv4_sequence(p, cur_b);
-      const int all = kv4_block_tiles(kv4_block_keys(s, group, kRows, cur_block));
-      pieces[2 * warp + 1] = Kv4Piece{cur_b, cur_head, cur_block, 2, unit_first_tile == 0, range_end - 1 - cur_tile, all};
-    }
+    write_piece(2 * warp + 1, reinterpret_cast<float*>(ring + warp * kStages * Cfg::kStageBytes));
+    if (lane == 0)
+      pieces[2 * warp + 1] = Kv4Piece{2, first_tile == 0, range + count - 1 - cur_tile, static_cast<unsigned>(kv4_block_tiles(cur_keys)),
+                                      cur_start, cur_block * kRows, min(kRows, cur_rows - cur_block * kRows), cur_head};
   }
   __syncthreads();
 
-  // ---- the warps' pieces, in order: an open piece belongs with those behind it up to the one that ends the sequence
-  auto piece_at = [&](int i) {
-    return pieces[i].kind == 1 ? params.slots + (2ll * gridDim.x + static_cast<long long>(blockIdx.x) * kWarps + i / 2) * Cfg::kPieceFloats
-                               : reinterpret_cast<const float*>(ring + (i / 2) * kStages * Cfg::kStageBytes);
+  // ---- the warps' pieces, in order: an open piece belongs with those behind it up to the one that ends the sequence.
+  // Groups of pieces as bit masks, the same in every warp.
+  const int kind = lane < 2 * kWarps ? pieces[lane].kind : 0;
+  const uint32_t present = __ballot_sync(0xffffffffu, kind != 0), ends = __ballot_sync(0xffffffffu, kind == 1);
+  if (!present) return;
+  const uint32_t last_end = ends ? 31 - __clz(ends) : 0;
+  const int groups = __popc(ends) + ((ends ? present >> last_end >> 1 : present) != 0 ? 1 : 0);
+  auto group_mask = [&](int piece) {                     // the pieces of this piece's group
+    const uint32_t below = (1u << piece) - 1, before = ends & below, behind = ends & ~below;
+    const uint32_t low = before ? ~((2u << (31 - __clz(before))) - 1) : ~0u;
+    const uint32_t high = behind ? (2u << (__ffs(behind) - 1)) - 1 : ~0u;
+    return present & low & high;
   };
-  auto write_out = [&](const Kv4Sequence& s, const Kv4Piece& unit, int row, int column, const float4& x) {
-    const int r = unit.block * kRows + row;
-    uint16_t* dst = p.out + (static_cast<int64_t>(s.start + r / group) * p.q_heads + unit.head * group + r % group) * kDim + column;
+  for (int i = thread; i < 2 * kWarps * kRows; i += kThreads) {
+    const int piece = i / kRows, row = i % kRows;
+    if (!(present >> piece & 1)) continue;
+    const uint32_t mask = group_mask(piece);
+    float most = -INFINITY, all = 0.f;
+    for (uint32_t rest = mask; rest; rest &= rest - 1) most = fmaxf(most, piece_m[__ffs(rest) - 1][row]);
+    if (piece == __ffs(mask) - 1) {
+      for (uint32_t rest = mask; rest; rest &= rest - 1) {
+        const int other = __ffs(rest) - 1;
+        const float l = piece_l[other][row];
+        all += l == 0.f ? 0.f : fast_exp2(piece_m[other][row] - most) * l;   // 0: saw no key (a NaN score makes the sum NaN, which is kept)
+      }
+      group_m[piece][row] = most;
+      group_l[piece][row] = all;
+    }
+    weights[piece][row] = piece_l[piece][row] == 0.f ? 0.f : fast_exp2(piece_m[piece][row] - most);
+  }
+  __syncthreads();
+  auto write_out = [&](const Kv4Piece& unit, int row, int column, const float4& x) {
+    const int r = unit.row + row, row_token = p.group.quotient(r);
+    uint16_t* dst = p.out + (static_cast<int64_t>(unit.start + row_token) * p.q_heads + unit.head * group + r - row_token * group) * kDim + column;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x, x.y), pack2(x.z, x.w));
   };
-  for (int at = 0; at < 2 * kWarps;) {
-    if (pieces[at].kind == 0) { ++at; continue; }
-    const int begin = at;
-    while (pieces[at].kind != 1 && ++at < 2 * kWarps) {}
-    const bool ends = at < 2 * kWarps;                   // else it goes on in the next CTA
-    const int end = ends ? ++at : at;
-    const Kv4Piece unit = pieces[begin];
-    const Kv4Sequence s = kv4_sequence(p, unit.b);
-    const int rows = min(kRows, s.rows * group - unit.block * kRows);
-    const bool closed = ends && unit.starts;
-    float* slot = params.slots + (2ll * blockIdx.x + (unit.starts ? 1 : 0)) * Cfg::kPieceFloats;
-    for (int e = thread; e < rows * (kDim / 4); e += kThreads) {
-      const int row = e / (kDim / 4), column = e % (kDim / 4) * 4;
-      float most = -INFINITY, all = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = begin; i < end; ++i)
-        if (pieces[i].kind) most = fmaxf(most, piece_at(i)[row]);
-      for (int i = begin; i < end; ++i) {
-        if (!pieces[i].kind) continue;
-        const float* from = piece_at(i);
-        const float part_sum = from[kRows + row];
-        if (part_sum == 0.f) continue;                   // saw no key (a NaN score makes its sum NaN, which is kept)
-        const float weight = fast_exp2(from[row] - most);
-        const float4 y = *reinterpret_cast<const float4*>(from + 2 * kRows + row * kDim + column);
-        all += weight * part_sum;
-        x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
-      }
-      if (closed) {
-        const float inverse = all == 0.f ? 0.f : 1.f / all;
-        write_out(s, unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
-      } else {
-        if (column == 0) { slot[row] = most; slot[kRows + row] = all; }
-        *reinterpret_cast<float4*>(slot + 2 * kRows + row * kDim + column) = x;
-      }
+  const float* const head_slots = params.slots + (2ll * gridDim.x + static_cast<long long>(blockIdx.x) * kWarps) * Cfg::kPieceFloats;
+  constexpr int kColumns = kDim / 4;
+  for (int i = thread; i < groups * kRows * kColumns; i += kThreads) {
+    const int column = i % kColumns * 4, row = i / kColumns % kRows;
+    uint32_t rest = present;                             // the group's first piece: the first behind the last end before it
+    for (int skip = i / (kColumns * kRows), n = 0; n < skip; ++n) rest &= ~((2u << (__ffs(rest & ends) - 1)) - 1);
+    const int piece = __ffs(rest) - 1;
+    const Kv4Piece unit = pieces[piece];
+    if (row >= unit.rows) continue;
+    const uint32_t mask = group_mask(piece);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (rest = mask; rest; rest &= rest - 1) {
+      const int other = __ffs(rest) - 1;
+      const float* from = other & 1 ? reinterpret_cast<const float*>(ring + (other / 2) * kStages * Cfg::kStageBytes)
+                                    : head_slots + (other / 2) * Cfg::kPieceFloats;
+      const float weight = weights[other][row];
+      if (weight == 0.f) continue;
+      const float4 y = *reinterpret_cast<const float4*>(from + row * kDim + column);
+      x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
     }
-    if (!closed && thread == 0) shared_units[unit.starts ? 1 : 0] = unit;
+    const float all = group_l[piece][row];
+    if (unit.starts && (mask & ends)) {
+      const float inverse = all == 0.f ? 0.f : 1.f / all;
+      write_out(unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+    } else {
+      float* slot = params.slots + (2ll * blockIdx.x + (unit.starts ? 1 : 0)) * Cfg::kPieceFloats;
+      if (column == 0) {
+        slot[row] = group_m[piece][row];
+        slot[kRows + row] = all;
+        if (row == 0) shared_units[unit.starts ? 1 : 0] = unit;
+      }
+      *reinterpret_cast<float4*>(slot + 2 * kRows + row * kDim + column) = x;
+    }
   }
   __syncthreads();
 
   // ---- sequences shared by several CTAs: the last to arrive joins the CTAs' slots in order and leaves the counter at zero
-  auto cta_of = [&](long long place) { return static_cast<int>(((place + 1) * workers - 1) / total / kWarps); };
+  auto cta_of = [&](unsigned place) -> int {
+    const unsigned of_longer = longer * (per_cta + 1);
+    return place < of_longer ? place / (per_cta + 1) : longer + (place - of_longer) / per_cta;
+  };
   if (thread < 2 && shared_units[thread].kind) {
     const Kv4Piece& unit = shared_units[thread];
     const int from = cta_of(unit.first), to = cta_of(unit.first + unit.tiles - 1);
@@ -633,11 +776,10 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     if (!comes_last[which]) continue;
     const Kv4Piece unit = shared_units[which];
     const int from = cta_of(unit.first), count_ctas = cta_of(unit.first + unit.tiles - 1) - from + 1;
-    const Kv4Sequence s = kv4_sequence(p, unit.b);
-    const int rows = min(kRows, s.rows * group - unit.block * kRows);
+    const int rows = unit.rows;
     const float* slots = params.slots + 2ll * from * Cfg::kPieceFloats;   // slot 1 of the first CTA, slot 0 of the others
     auto slot_of = [&](int i) { return slots + (2ll * i + (i == 0 ? 1 : 0)) * Cfg::kPieceFloats; };
-    float* weights = reinterpret_cast<float*>(ring);                      // [CTA][row]; the pieces in the ring are done with
+    float* cta_weights = reinterpret_cast<float*>(ring);                  // [CTA][row]; the pieces in the ring are done with
     for (int row = warp; row < rows; row += kWarps) {
       float most = -INFINITY, all = 0.f;
       for (int i = lane; i < count_ctas; i += 32) most = fmaxf(most, __ldcg(slot_of(i) + row));
@@ -646,7 +788,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       for (int i = lane; i < count_ctas; i += 32) {
         const float part_sum = __ldcg(slot_of(i) + kRows + row);
         const float weight = part_sum == 0.f ? 0.f : fast_exp2(__ldcg(slot_of(i) + row) - most);
-        weights[i * kRows + row] = weight;
+        cta_weights[i * kRows + row] = weight;
         all += weight * part_sum;
       }
 #pragma unroll
@@ -659,12 +801,12 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int i = 0; i < count_ctas; ++i) {
-        const float weight = weights[i * kRows + row];
+        const float weight = cta_weights[i * kRows + row];
         const float4 y = __ldcg(reinterpret_cast<const float4*>(slot_of(i) + 2 * kRows + row * kDim + column));
         x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
       }
       const float inverse = inverse_sums[row];
-      write_out(s, unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+      write_out(unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
     }
     __syncthreads();
   }
