@@ -15,6 +15,7 @@
 #include "gemm_tcgen05.cuh"
 #include "gemv_w8a16.cuh"
 #include "kv4_attention.cuh"
+#include "kv4_prompt.cuh"
 #include "kv4_rows.cuh"
 #include "kv4_single.cuh"
 #include "q8_block.cuh"
@@ -887,6 +888,45 @@ int launch_kv4_single(const Kv4AttendParams& a, void* workspace, int most_rows, 
                                      : launch_kv4_single_q<kDim, 2>(a, workspace, most_rows, stream);
 }
 
+// Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys and a second kernel joins.
+template <int kDim>
+int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
+  using Cfg = Kv4PromptConfig<kDim>;
+  static std::atomic<uint64_t> raised{0};
+  const cudaError_t err = ensure_smem(kv4_prompt_kernel<kDim>, Cfg::kSmemBytes, raised);
+  if (err != cudaSuccess) return static_cast<int>(err);
+  const long long all_rows = static_cast<long long>(a.tokens) * a.group.d;
+  long long sequences = all_rows / (most_rows + 1);       // that have more rows than most_rows
+  if (sequences > a.batch) sequences = a.batch;
+  const long long tiles = all_rows / Cfg::kRows + sequences;   // no more row tiles than that
+  if (tiles == 0) return 0;
+  if (tiles > 0x7fffffffll) return kInvalid;
+  const long long key_tiles = ((static_cast<long long>(a.width) << a.page_shift) + Cfg::kKeys - 1) / Cfg::kKeys;
+  long long splits = sm_count() / (tiles * a.kv_heads);
+  if (splits > key_tiles / 4) splits = key_tiles / 4;
+  if (splits > 16) splits = 16;
+  const long long slot = static_cast<long long>(Cfg::kRows) * (kDim + 2) * 4;
+  while (splits > 1 && kKv4CounterBytes + tiles * a.kv_heads * splits * slot > kKv4WorkspaceBytes) --splits;
+  Kv4PromptParams p;
+  p.a = a;
+  p.splits = splits > 1 ? static_cast<int>(splits) : 1;
+  p.partial = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv4CounterBytes) : nullptr;
+  p.most_rows = most_rows;
+  const int code = launch_pdl(kv4_prompt_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, p.splits), Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  if (code || p.splits == 1) return code;
+  return launch_pdl(kv4_prompt_join_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, 8), 256, 0, stream, p);
+}
+// Sequences with few rows go to the kernel for generated tokens, the others to the one for prompts; which they are is
+// only known on the device, so each kernel passes over the other's. No sequence has more than one row (or the rows
+// happen to be spread unevenly) when there are no more rows than sequences: one kernel.
+constexpr int kKv4FewRows = 16;
+template <int kDim>
+int launch_kv4_attention(const Kv4AttendParams& a, void* workspace, ci8_stream_t stream) {
+  if (a.tokens <= a.batch) return launch_kv4_single<kDim>(a, workspace, 0x7fffffff, stream);
+  const int code = launch_kv4_single<kDim>(a, workspace, kKv4FewRows, stream);
+  return code ? code : launch_kv4_prompt<kDim>(a, workspace, kKv4FewRows, stream);
+}
+
 }  // namespace
 
 // ====================================================================== C ABI
@@ -1360,8 +1400,8 @@ int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, cons
   p.tokens = tokens; p.batch = batch; p.width = width; p.q_heads = q_heads; p.kv_heads = kv_heads;
   p.page_shift = shift; p.pages = pages; p.scale_log2 = scale * 1.4426950408889634f;
   p.group = Kv4Divisor::of(static_cast<unsigned>(q_heads / kv_heads));
-  return dim == 64 ? launch_kv4_single<64>(p, workspace, 0x7fffffff, stream)
-         : dim == 128 ? launch_kv4_single<128>(p, workspace, 0x7fffffff, stream) : launch_kv4_single<256>(p, workspace, 0x7fffffff, stream);
+  return dim == 64 ? launch_kv4_attention<64>(p, workspace, stream)
+         : dim == 128 ? launch_kv4_attention<128>(p, workspace, stream) : launch_kv4_attention<256>(p, workspace, stream);
 }
 
 }  // extern "C"

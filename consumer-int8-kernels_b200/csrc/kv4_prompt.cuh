@@ -1,0 +1,637 @@
+// Attention of many query rows per sequence (prompts, chunks of prompts) over the 4-bit key/value cache, on tcgen05.
+//
+// A CTA takes up to 256 query rows of one key head (a row is a token and one of the query heads that share the key
+// head, so their keys are unpacked once), as tiles of 128: two for dim 64 and 128, one for dim 256 (512 TMEM columns
+// hold the scores and outputs of no more). It walks the keys in tiles of 128 (64 for dim 256):
+//   unpack warps   codes from global memory (a half-step ahead, in registers) -> BF16 code - zero, exact small integers,
+//                  into the 128-byte-swizzled operand tiles; scales beside them as FP32
+//   MMA warp       S = Q K^T (both from shared memory), O += P V (P from TMEM)
+//   softmax warps  one thread per row: S * key scale, running maximum and sum, weights * value scale rounded to BF16
+//                  into the columns of S. The output is scaled only when a row's maximum has grown by more than 2^8.
+// The components of a word come out of the unpacking as 0 4 1 5 2 6 3 7; the queries are stored in that order and the
+// output is put back. The tensor pipe needs 4 * dim * 256 / 8192 cycles per key, the exponentials 256 / 16: equal at
+// dim 128, so both have to run all the time; the two query tiles take turns on either.
+#pragma once
+#include "kv4_attention.cuh"
+
+namespace ci8 {
+
+template <int kDim>
+struct Kv4PromptConfig {
+  static constexpr int kQTiles = kDim == 256 ? 1 : 2;
+  static constexpr int kRows = 128 * kQTiles;            // query rows of a CTA
+  static constexpr int kKeys = kDim == 256 ? 64 : 128;   // keys of a tile
+  static constexpr int kUnpackGroups = kDim == 256 ? 2 : 1;
+  static constexpr int kThreads = 512;                   // softmax, unpack and MMA warpgroups
+  static constexpr int kQBytes = 128 * kDim * 2;
+  static constexpr int kTileBytes = kKeys * kDim * 2;
+  static constexpr int kStages = 2;
+  static constexpr int kSmemBytes = kQTiles * kQBytes + 2 * kStages * kTileBytes + 1024;
+  // registers per thread after the hand-over; together 512 * 128
+  static constexpr int kSoftmaxRegs = 192;
+  static constexpr int kUnpackRegs = kDim == 256 ? 120 : 88;
+  static constexpr int kMmaRegs = 40;
+  static_assert(kQTiles * kSoftmaxRegs + kUnpackGroups * kUnpackRegs + kMmaRegs <= 512 && kSoftmaxRegs > 128 && kUnpackRegs < 128 && kMmaRegs < 128,
+                "what is taken has been given back, and only a smaller number is a giving back");
+};
+
+struct Kv4PromptParams {
+  Kv4AttendParams a;
+  float* partial;             // [tile][key head][split][maximum, sum, output of every row], null: one split
+  int splits;
+  int most_rows;              // sequences with no more query rows than this belong to another kernel
+};
+
+// Scales are read by the softmax warps, up to two tiles behind the unpacking: the values of tile j + 2 are not unpacked
+// before the second product of tile j, whose weights come after its scales were read. So tile j + 4 may take tile j's slot,
+// and the marks of tile j + 4 can be cleared while tile j's are being set.
+constexpr int kKv4ScaleSlots = 4;
+constexpr int kKv4MarkSlots = 8;
+
+__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, bool b_transposed) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+// Operand tiles are stored as segments of 64 components: rows of 128 bytes, swizzled. The same tile serves as keys
+// (K-major: components along K) and as values (components along N: `segment` is the distance between segments).
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr, uint32_t segment) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(segment >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+               "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+               "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
+      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float kv4_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// The sequence and the place in it of row tile `index` (tiles of `rows` query rows, counted over the sequences that have
+// more than most_rows); all lanes of a warp together. Returns the number of tiles there are.
+struct Kv4PromptTile {
+  int b, tile;
+};
+__device__ __forceinline__ int kv4_prompt_tile(const Kv4AttendParams& p, int rows, int most_rows, int index, Kv4PromptTile& found) {
+  const int lane = threadIdx.x % 32;
+  found = {-1, 0};
+  int before = 0;
+  for (int base = 0; base < p.batch; base += 32) {
+    const int b = base + lane;
+    int tiles = 0;
+    if (b < p.batch) {
+      const int q_rows = kv4_sequence(p, b).rows * static_cast<int>(p.group.d);
+      if (q_rows > most_rows) tiles = (q_rows + rows - 1) / rows;
+    }
+    int scan = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xffffffffu, scan, d);
+      if (lane >= d) scan += other;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, index >= before + scan - tiles && index < before + scan);
+    if (hit) {
+      const int from = __ffs(hit) - 1;
+      found = {base + from, index - (before + __shfl_sync(0xffffffffu, scan - tiles, from))};
+    }
+    before += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  return before;
+}
+
+// A bounded wait of a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, int parity, int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort));
+}
+
+template <int kDim>
+__global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParams params) {
+  using Cfg = Kv4PromptConfig<kDim>;
+  constexpr int kQTiles = Cfg::kQTiles, kKeys = Cfg::kKeys, kStages = Cfg::kStages;
+  constexpr int kSegments = kDim / 64;                   // of 64 components, 128 bytes a row
+  constexpr int kSoftmaxGroups = kQTiles;
+  constexpr uint32_t kOutputColumn = 256;
+  extern __shared__ uint8_t dynamic_smem[];
+  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2], bar_done[2], bar_k[kStages], bar_k_free[kStages], bar_v[kStages], bar_v_free[kStages];
+  __shared__ __align__(8) uint64_t bar_scale_k[kKv4ScaleSlots], bar_scale_v[kKv4ScaleSlots];
+  __shared__ __align__(16) float scale_k[kKv4ScaleSlots][kKeys], scale_v[kKv4ScaleSlots][kKeys];
+  __shared__ uint32_t hidden[kKv4MarkSlots][kKeys / 32];   // keys of the tile on a page that could not be followed
+  __shared__ int any_hidden[kKv4MarkSlots];
+  __shared__ uint32_t tmem_base;
+  __shared__ int abort_flag, tile_info[2];
+  const Kv4AttendParams& p = params.a;
+  const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32, warpgroup = warp / 4;
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* const q_smem = smem;
+  uint8_t* const k_smem = smem + kQTiles * Cfg::kQBytes;
+  uint8_t* const v_smem = k_smem + kStages * Cfg::kTileBytes;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(smem_u32(&bar_q), 128 * kQTiles);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&bar_s[i]), 1);
+        mbar_init(smem_u32(&bar_p[i]), 128);
+        mbar_init(smem_u32(&bar_done[i]), 1);
+      }
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(smem_u32(&bar_k[i]), 128);
+        mbar_init(smem_u32(&bar_k_free[i]), 1);
+        mbar_init(smem_u32(&bar_v[i]), 128);
+        mbar_init(smem_u32(&bar_v_free[i]), 1);
+      }
+      for (int i = 0; i < kKv4ScaleSlots; ++i) {
+        mbar_init(smem_u32(&bar_scale_k[i]), 128);
+        mbar_init(smem_u32(&bar_scale_v[i]), 128);
+      }
+      abort_flag = 0;
+    }
+    if (lane < kKv4MarkSlots) {
+      any_hidden[lane] = 0;
+      for (int c = 0; c < kKeys / 32; ++c) hidden[lane][c] = 0;
+    }
+    __syncwarp();
+    fence_barrier_init();
+    tmem_alloc<1>(smem_u32(&tmem_base), 512);
+    tmem_relinquish<1>();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 1) {
+    // the last row tiles see the most keys: they go first
+    Kv4PromptTile found;
+    const int all = kv4_prompt_tile(p, Cfg::kRows, params.most_rows, -1, found);
+    const int index = all - 1 - static_cast<int>(blockIdx.x);
+    if (index >= 0) kv4_prompt_tile(p, Cfg::kRows, params.most_rows, index, found);
+    if (lane == 0) {
+      tile_info[0] = index >= 0 ? found.b : -1;
+      tile_info[1] = found.tile;
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_base;
+  const int b = tile_info[0], first_row = tile_info[1] * Cfg::kRows, head = blockIdx.y, split = blockIdx.z;
+  const int group = p.group.d;
+
+  if (b >= 0) {
+    const Kv4Sequence seq = kv4_sequence(p, b);
+    const int all_rows = seq.rows * group;
+    const int last_row = min(all_rows, first_row + Cfg::kRows) - 1;
+    const int keys = max(0, seq.keys - seq.rows + p.group.quotient(last_row) + 1);   // that the CTA's last row sees
+    const int all_tiles = (keys + kKeys - 1) / kKeys;
+    const int begin = static_cast<int>(static_cast<long long>(all_tiles) * split / params.splits);
+    const int end = static_cast<int>(static_cast<long long>(all_tiles) * (split + 1) / params.splits);
+    const int tiles = end - begin;
+
+    if (warpgroup < kSoftmaxGroups) {
+      // ================================================================ softmax: one thread per query row
+      setmaxnreg_inc<Cfg::kSoftmaxRegs>();
+      const int t = warpgroup, row_in_tile = thread % 128, row = first_row + 128 * t + row_in_tile;
+      {
+        // the tile's queries, in the unpacked codes' order
+        constexpr int kPieces = kDim / 8;
+        uint8_t* const tile = q_smem + t * Cfg::kQBytes;
+        for (int i = row_in_tile; i < 128 * kPieces; i += 128) {
+          const int r = i / kPieces, piece = i % kPieces, q_row = first_row + 128 * t + r;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (q_row < all_rows) {
+            const int token = p.group.quotient(q_row);
+            w = *reinterpret_cast<const uint4*>(p.q + (seq.start + token) * p.q_stride +
+                                                static_cast<int64_t>(head * group + q_row - token * group) * kDim + 8 * piece);
+          }
+          const uint4 turned = make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
+                                          __byte_perm(w.y, w.w, 0x7632));
+          *reinterpret_cast<uint4*>(tile + (piece / 8) * (128 * 128) + r * 128 + ((piece % 8) ^ (r & 7)) * 16) = turned;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&bar_q));
+      }
+      const int token = p.group.quotient(row);
+      const int limit = row < all_rows ? max(0, seq.keys - seq.rows + token + 1) : 0;
+      const int least = __reduce_min_sync(0xffffffffu, limit);
+      const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+      const uint32_t output = tmem + lanes + kOutputColumn + t * kDim;
+      float m = -INFINITY;
+      float2 sum2 = make_float2(0.f, 0.f);
+      bool fine = true;
+      for (int j = 0; j < tiles && fine; ++j) {
+        const int buffer = kQTiles == 2 ? t : j & 1;
+        const uint32_t scores = tmem + lanes + 128 * buffer;
+        const int slot = j % kKv4ScaleSlots, slot_parity = j / kKv4ScaleSlots & 1;
+        const int parity = kQTiles == 2 ? j & 1 : j >> 1 & 1;
+        fine = warp_wait(&bar_s[buffer], parity, &abort_flag) && warp_wait(&bar_scale_k[slot], slot_parity, &abort_flag);
+        if (!fine) break;
+        tcgen05_fence_after();
+        uint32_t s[kKeys / 32][32];
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(scores + 32 * c, s[c]);
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_wait_for(s[c]);
+        const int first_key = (begin + j) * kKeys;
+        const bool masked = first_key + kKeys > least || any_hidden[j % kKv4MarkSlots];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(&scale_k[slot][32 * c + i]);
+            const float2 lo = __fmul2_rn(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), make_float2(k.x, k.y));
+            const float2 hi = __fmul2_rn(make_float2(__uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3])), make_float2(k.z, k.w));
+            s[c][i] = __float_as_uint(lo.x);
+            s[c][i + 1] = __float_as_uint(lo.y);
+            s[c][i + 2] = __float_as_uint(hi.x);
+            s[c][i + 3] = __float_as_uint(hi.y);
+          }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < kKeys / 32; ++c) {
+            const int seen = min(32, max(0, limit - first_key - 32 * c));
+            const uint32_t shown = (seen == 32 ? ~0u : (1u << seen) - 1) & ~hidden[j % kKv4MarkSlots][c];
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(shown >> i & 1)) s[c][i] = 0xff800000u;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c][i]));
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+        if (__any_sync(0xffffffffu, most > m + 8.f)) {
+          const float next = fmaxf(m, most);
+          const float keep = next == -INFINITY ? 1.f : kv4_exp2(m - next);
+          m = next;
+          sum2.x *= keep;
+          sum2.y *= keep;
+          if (j > 0) {
+            // Two query tiles: these scores were issued behind the product that last wrote the output, which is
+            // complete. One: that product may still be running.
+            if (kQTiles == 1) {
+              fine = warp_wait(&bar_done[1], (j - 1) & 1, &abort_flag);
+              if (!fine) break;
+              tcgen05_fence_after();
+            }
+#pragma unroll 1
+            for (int c = 0; c < kDim; c += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32(output + c, o);
+              tmem_ld_wait_for(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+              tmem_st_32x32(output + c, o);
+            }
+          }
+        }
+        fine = warp_wait(&bar_scale_v[slot], slot_parity, &abort_flag);
+        if (!fine) break;
+        const float base = m == -INFINITY ? 0.f : -m;
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), base2 = make_float2(base, base);
+#pragma unroll
+        for (int h = 0; h < kKeys / 64; ++h) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 4) {
+            uint32_t(&from)[32] = s[2 * h + i / 32];
+            const float4 v = *reinterpret_cast<const float4*>(&scale_v[slot][64 * h + i]);
+            float2 x = __ffma2_rn(make_float2(__uint_as_float(from[i % 32]), __uint_as_float(from[i % 32 + 1])), scale2, base2);
+            float2 y = __ffma2_rn(make_float2(__uint_as_float(from[i % 32 + 2]), __uint_as_float(from[i % 32 + 3])), scale2, base2);
+            x = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
+            y = make_float2(kv4_exp2(y.x), kv4_exp2(y.y));
+            sum2 = __fadd2_rn(sum2, x);
+            sum2 = __fadd2_rn(sum2, y);
+            x = __fmul2_rn(x, make_float2(v.x, v.y));
+            y = __fmul2_rn(y, make_float2(v.z, v.w));
+            packed[i / 2] = pack2(x.x, x.y);
+            packed[i / 2 + 1] = pack2(y.x, y.y);
+          }
+          tmem_st_32x32(scores + 32 * h, packed);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        mbar_arrive(smem_u32(&bar_p[buffer]));
+      }
+      // ---- output
+      if (fine && tiles > 0) fine = warp_wait(&bar_done[t], 0, &abort_flag);
+      tcgen05_fence_after();
+      const float sum = sum2.x + sum2.y;
+      if (params.partial) {
+        float* slot = params.partial + (((static_cast<int64_t>(blockIdx.x) * p.kv_heads + head) * params.splits + split) * Cfg::kRows + 128 * t) * (kDim + 2);
+        slot[row_in_tile] = m;                             // [128 maxima][128 sums][128 outputs]
+        slot[128 + row_in_tile] = sum;
+        float* dst = slot + 256 + row_in_tile * kDim;
+        if (tiles > 0 && fine) {
+#pragma unroll 1
+          for (int c = 0; c < kDim; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(output + c, o);
+            tmem_ld_wait_for(o);
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(o[i], o[i + 2], o[i + 4], o[i + 6]);
+              *reinterpret_cast<uint4*>(dst + c + i + 4) = make_uint4(o[i + 1], o[i + 3], o[i + 5], o[i + 7]);
+            }
+          }
+        }
+      } else {
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t* dst = p.out + (static_cast<int64_t>(seq.start + token) * p.q_heads + head * group + row - token * group) * kDim;
+#pragma unroll 1
+        for (int c = 0; c < kDim; c += 32) {
+          uint32_t o[32];
+          if (tiles > 0 && fine) {
+            tmem_ld_32x32(output + c, o);
+            tmem_ld_wait_for(o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
+          if (row < all_rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[i + e]) * inverse;
+              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(pack2(x[0], x[2]), pack2(x[4], x[6]), pack2(x[1], x[3]), pack2(x[5], x[7]));
+            }
+          }
+        }
+      }
+    } else if (warpgroup < 3) {
+      // ================================================================ unpacking
+      setmaxnreg_dec<Cfg::kUnpackRegs>();
+      // One group unpacks keys and values in turn; two groups take one each.
+      const int side_first = Cfg::kUnpackGroups == 2 ? warpgroup - kSoftmaxGroups : 0;
+      constexpr int kSteps = Cfg::kUnpackGroups == 2 ? 1 : 2;          // half-steps (sides) per tile of keys
+      // Lane mapping: eight neighbouring lanes take eight rows of one piece of 16 code bytes (conflict-free stores), the
+      // four such octets the pieces (dim 128), half the pieces (256), or the pieces of two runs of rows (64).
+      constexpr int kPasses = kDim == 64 ? 2 : kDim == 128 ? 4 : 2;
+      constexpr int kLoads = kDim == 256 ? 2 : 1;                      // pieces of a row a lane takes
+      constexpr int kPassRows = kKeys / kPasses;
+      const int octet = lane / 8;
+      const int lane_row = (kDim == 64 ? 16 * (warp % 4) + 8 * (octet / 2) : 8 * (warp % 4)) + lane % 8;
+      const int lane_piece = kDim == 64 ? octet % 2 : octet;
+      const int page = 1 << p.page_shift;
+      const int64_t block_bytes = kv4_block_bytes(page, kDim);
+      const int32_t* const table = p.block_table + static_cast<int64_t>(b) * p.width;
+      // page numbers of the keys ahead: 32 in the lanes and the next 32 behind them
+      int window_first = begin * kKeys >> p.page_shift;
+      auto load_window = [&](int from) {
+        const int64_t index = static_cast<int64_t>(from) + lane;
+        return (index << p.page_shift) < keys ? table[index] : -1;
+      };
+      int window = load_window(window_first), window_next = load_window(window_first + 32);
+      uint4 codes[kPasses][kLoads];
+      uint32_t pairs[kPasses];                           // bit 31 of a pair's scale marks a page that cannot be followed
+      auto load = [&](int step) {
+        const int tile = begin + step / kSteps, side = kSteps == 2 ? step & 1 : side_first;
+        while ((((tile + 1) * kKeys - 1) >> p.page_shift) - window_first >= 32 + 32) {
+          window_first += 32;
+          window = window_next;
+          window_next = load_window(window_first + 32);
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          const int key = tile * kKeys + kPassRows * i + lane_row;
+          const int index = (key >> p.page_shift) - window_first;
+          const int low = __shfl_sync(0xffffffffu, window, index & 31), high = __shfl_sync(0xffffffffu, window_next, index & 31);
+          const int id = index < 32 ? low : high;
+          const bool wanted = key < keys, good = wanted && static_cast<unsigned>(id) < static_cast<unsigned>(p.pages);
+#pragma unroll
+          for (int n = 0; n < kLoads; ++n) codes[i][n] = make_uint4(0, 0, 0, 0);
+          pairs[i] = wanted ? 0x8000u : 0u;
+          if (good) {
+            const uint8_t* src = p.cache + ((static_cast<int64_t>(id) * kKv4Side + side) * p.kv_heads + head) * block_bytes;
+            const int at = key & (page - 1);
+            pairs[i] = __ldcg(reinterpret_cast<const unsigned*>(src + page * (kDim / 2) + 4 * at)) & 0xffff7fffu;
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n)
+              codes[i][n] = __ldcg(reinterpret_cast<const uint4*>(src + at * (kDim / 2) + 16 * (lane_piece + 4 * n)));
+          }
+        }
+      };
+      const int steps = tiles * kSteps;
+      bool fine = true;
+      if (steps > 0) load(0);
+      for (int step = 0; step < steps; ++step) {
+        const int j = step / kSteps, side = kSteps == 2 ? step & 1 : side_first;
+        const int stage = j % kStages, slot = j % kKv4ScaleSlots;
+        uint64_t* const full = side ? bar_v : bar_k;
+        uint64_t* const empty = side ? bar_v_free : bar_k_free;
+        uint4 now[kPasses][kLoads];
+        uint32_t now_pairs[kPasses];
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          now_pairs[i] = pairs[i];
+#pragma unroll
+          for (int n = 0; n < kLoads; ++n) now[i][n] = codes[i][n];
+        }
+        if (step + 1 < steps) load(step + 1);
+        if (j >= kStages) fine = warp_wait(&empty[stage], (j / kStages - 1) & 1, &abort_flag);
+        if (!fine) break;
+        uint8_t* const tile = (side ? v_smem : k_smem) + stage * Cfg::kTileBytes;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          const int row = kPassRows * i + lane_row;
+          const bool marked = now_pairs[i] & 0x8000u;
+          const float zero = 128.f + bf16_hi(now_pairs[i]);
+          const uint32_t zeros = pack2(zero, zero);
+          if (lane_piece == 0) {
+            if (side) scale_v[slot][row] = marked ? 0.f : bf16_lo(now_pairs[i]);
+            else scale_k[slot][row] = marked ? 0.f : bf16_lo(now_pairs[i]);
+          }
+          bad |= marked;
+#pragma unroll
+          for (int n = 0; n < kLoads; ++n) {
+            const int piece = lane_piece + 4 * n;
+            const uint32_t words[4] = {now[i][n].x, now[i][n].y, now[i][n].z, now[i][n].w};
+            uint8_t* const segment = tile + (piece / 2) * (kKeys * 128) + row * 128;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              uint32_t v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] = ((words[w] >> (4 * e)) & 0x000f000fu) | 0x43004300u;
+                asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v[e]) : "r"(zeros));
+              }
+              *reinterpret_cast<uint4*>(segment + (((piece % 2) * 4 + w) ^ (row & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        if (side == 0) {
+          if (warp % 4 == 0) {
+            const int clear = (j + kKv4ScaleSlots) % kKv4MarkSlots;
+            if (lane < kKeys / 32) hidden[clear][lane] = 0;
+            if (lane == 0) any_hidden[clear] = 0;
+          }
+          if (bad) {
+            any_hidden[j % kKv4MarkSlots] = 1;
+            atomicOr(&g_ci8_status, kStatusBadIndex);
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+              const int row = kPassRows * i + lane_row;
+              if (now_pairs[i] & 0x8000u) atomicOr(&hidden[j % kKv4MarkSlots][row / 32], 1u << (row % 32));
+            }
+          }
+          mbar_arrive(smem_u32(&bar_scale_k[slot]));
+        } else {
+          mbar_arrive(smem_u32(&bar_scale_v[slot]));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&full[stage]));
+      }
+    } else {
+      setmaxnreg_dec<Cfg::kMmaRegs>();
+      if (warp == 12 && tiles > 0) {
+        // ================================================================ MMA issue
+        constexpr uint32_t kIdescS = idesc_bf16(128, kKeys, false), kIdescO = idesc_bf16(128, kDim, true);
+        const uint32_t q_at = smem_u32(q_smem), k_at = smem_u32(k_smem), v_at = smem_u32(v_smem);
+        auto scores = [&](int t, int buffer, int stage) {
+          if (elect_one()) {
+#pragma unroll
+            for (int s = 0; s < kSegments; ++s)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_bf16_ss(tmem + 128 * buffer, smem_desc_sw128(q_at + t * Cfg::kQBytes + s * (128 * 128)) + 2 * k,
+                            smem_desc_sw128(k_at + stage * Cfg::kTileBytes + s * (kKeys * 128)) + 2 * k, kIdescS, s + k > 0);
+            mma_commit(smem_u32(&bar_s[buffer]));
+          }
+          __syncwarp();
+        };
+        auto outputs = [&](int t, int buffer, int stage, bool accumulate) {
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_bf16_ts(tmem + kOutputColumn + t * kDim, tmem + 128 * buffer + 8 * k,
+                          smem_desc_sw128_mn(v_at + stage * Cfg::kTileBytes + k * 2048, kKeys * 128), kIdescO, accumulate || k > 0);
+          }
+          __syncwarp();
+        };
+        auto commit = [&](uint64_t* bar) {
+          if (elect_one()) mma_commit(smem_u32(bar));
+          __syncwarp();
+        };
+        bool fine = warp_wait(&bar_q, 0, &abort_flag);
+        tcgen05_fence_after();
+        if constexpr (kQTiles == 2) {
+          for (int j = 0; j <= tiles && fine; ++j) {
+            for (int t = 0; t < 2 && fine; ++t) {
+              if (j > 0) {
+                const int stage = (j - 1) % kStages;
+                if (t == 0) fine = warp_wait(&bar_v[stage], (j - 1) / kStages & 1, &abort_flag);
+                fine = fine && warp_wait(&bar_p[t], (j - 1) & 1, &abort_flag);
+                if (!fine) break;
+                tcgen05_fence_after();
+                outputs(t, t, stage, j > 1);
+                if (t == 1) commit(&bar_v_free[stage]);
+                if (j == tiles) commit(&bar_done[t]);
+              }
+              if (j < tiles) {
+                const int stage = j % kStages;
+                if (t == 0) {
+                  fine = warp_wait(&bar_k[stage], j / kStages & 1, &abort_flag);
+                  if (!fine) break;
+                  tcgen05_fence_after();
+                }
+                scores(t, t, stage);
+                if (t == 1) commit(&bar_k_free[stage]);
+              }
+            }
+          }
+        } else {
+          for (int j = 0; j <= tiles && fine; ++j) {
+            if (j < tiles) {
+              const int stage = j % kStages;
+              fine = warp_wait(&bar_k[stage], j / kStages & 1, &abort_flag);
+              if (!fine) break;
+              tcgen05_fence_after();
+              scores(0, j & 1, stage);
+              commit(&bar_k_free[stage]);
+            }
+            if (j > 0) {
+              const int stage = (j - 1) % kStages, buffer = (j - 1) & 1;
+              fine = warp_wait(&bar_v[stage], (j - 1) / kStages & 1, &abort_flag) &&
+                     warp_wait(&bar_p[buffer], (j - 1) >> 1 & 1, &abort_flag);
+              if (!fine) break;
+              tcgen05_fence_after();
+              outputs(0, buffer, stage, j > 1);
+              commit(&bar_v_free[stage]);
+              commit(&bar_done[j == tiles ? 0 : 1]);
+            }
+          }
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc<1>(tmem, 512);
+}
+
+// Joins the splits of a row tile: grid (row tiles, key heads), in the order of the splits.
+template <int kDim>
+__global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const Kv4PromptParams params) {
+  using Cfg = Kv4PromptConfig<kDim>;
+  __shared__ int tile_info[2];
+  const Kv4AttendParams& p = params.a;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (threadIdx.x < 32) {
+    Kv4PromptTile found;
+    const int all = kv4_prompt_tile(p, Cfg::kRows, params.most_rows, -1, found);
+    const int index = all - 1 - static_cast<int>(blockIdx.x);
+    if (index >= 0) kv4_prompt_tile(p, Cfg::kRows, params.most_rows, index, found);
+    if (threadIdx.x == 0) {
+      tile_info[0] = index >= 0 ? found.b : -1;
+      tile_info[1] = found.tile;
+    }
+  }
+  __syncthreads();
+  const int b = tile_info[0], first_row = tile_info[1] * Cfg::kRows, head = blockIdx.y, group = p.group.d;
+  if (b < 0) return;
+  const Kv4Sequence seq = kv4_sequence(p, b);
+  const int rows = min(Cfg::kRows, seq.rows * group - first_row);
+  const float* base = params.partial + (static_cast<int64_t>(blockIdx.x) * p.kv_heads + head) * params.splits * Cfg::kRows * (kDim + 2);
+  for (int e = threadIdx.x + 256 * blockIdx.z; e < rows * (kDim / 4); e += 256 * gridDim.z) {
+    const int row = e / (kDim / 4), column = e % (kDim / 4) * 4;
+    auto piece = [&](int s) { return base + (static_cast<int64_t>(s) * Cfg::kRows + row / 128 * 128) * (kDim + 2); };
+    float most = -INFINITY, all = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < params.splits; ++s) most = fmaxf(most, piece(s)[row % 128]);
+    for (int s = 0; s < params.splits; ++s) {
+      const float sum = piece(s)[128 + row % 128];
+      if (sum == 0.f) continue;                          // saw no key (a NaN score makes its sum NaN, which is kept)
+      const float weight = kv4_exp2(piece(s)[row % 128] - most);
+      const float4 y = *reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column);
+      all += weight * sum;
+      x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
+    }
+    const float inverse = all == 0.f ? 0.f : 1.f / all;
+    const int r = first_row + row, token = p.group.quotient(r);
+    uint16_t* dst = p.out + (static_cast<int64_t>(seq.start + token) * p.q_heads + head * group + r - token * group) * kDim + column;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inverse, x.y * inverse), pack2(x.z * inverse, x.w * inverse));
+  }
+}
+
+}  // namespace ci8

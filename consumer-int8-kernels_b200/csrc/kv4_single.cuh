@@ -117,9 +117,31 @@ __device__ __forceinline__ void lds_words(const uint8_t* at, uint32_t (&w)[4]) {
   const uint4 v = *reinterpret_cast<const uint4*>(at);
   w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
 }
-// Sixteen bytes to shared memory past the registers and the L1; what is beyond `bytes` is filled with zeros.
+// Sixteen bytes to shared memory past the registers and the L1, at a fixed offset from both addresses.
+template <int kDst, int kSrc>
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(kDst), "n"(kSrc) : "memory");
+}
+// The same with what is beyond `bytes` filled with zeros.
+template <int kDst, int kSrc>
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(kDst), "n"(kSrc) : "memory");
+}
+// Code rows of half a tile, 512 bytes at a time: kCopies copies at kDst + 512 * i.
+template <int kCopies, int kDst, int i = 0>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src) {
+  if constexpr (i < kCopies) {
+    copy16<kDst + 512 * i, 512 * i>(dst, src);
+    copy_rows<kCopies, kDst, i + 1>(dst, src);
+  }
+}
+// Of those rows the first `rows`; the lane's row of the first copy is lane_row, and a copy covers kPerCopy.
+template <int kCopies, int kDst, int kPerCopy, int i = 0>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src, int rows, int lane_row) {
+  if constexpr (i < kCopies) {
+    copy16<kDst + 512 * i, 512 * i>(dst, src, lane_row + i * kPerCopy < rows ? 16 : 0);
+    copy_rows<kCopies, kDst, kPerCopy, i + 1>(dst, src, rows, lane_row);
+  }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -243,12 +265,16 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   // ---- the loader's side of the ring: the tiles of the range in order, copied by the lanes in pieces of 16 bytes (a tile
   // touches one page, or two of 16 tokens); the lanes hold the next 32 page numbers of the sequence
   const int page = 1 << p.page_shift;
-  const int64_t block_bytes = kv4_block_bytes(page, kDim), page_bytes = block_bytes * kKv4Side * p.kv_heads;
+  const unsigned block_bytes = page * (kDim / 2 + 4), page_bytes = block_bytes * kKv4Side * p.kv_heads;   // at most 70 MB
   const uint32_t ring_base = smem_u32(ring) + warp * kStages * Cfg::kStageBytes;
   const bool two_parts = page < kKv4Tile;
   constexpr int kRowPieces = kDim / 32;                  // 16-byte pieces of a code row
   const int lane_row = lane / kRowPieces;                // the lane's row among those one copy instruction covers
   const uint32_t lane_code = ring_base + 16 * lane;
+  const unsigned value_lane = p.kv_heads * block_bytes + 16 * lane;
+  const int pair_token = 4 * (lane & 7);
+  const unsigned pair_offset = page * (kDim / 2) + 4 * pair_token + (lane & 8 ? p.kv_heads * block_bytes : 0);
+  const uint32_t pair_dst = ring_base + Cfg::kCodeBytes + 4 * pair_token + (lane & 8 ? Cfg::kCodeBytes + Cfg::kPairBytes : 0);
   const uint8_t* head_src = nullptr;
   int window = -1, window_first = 0;
   auto load_window = [&]() {
@@ -257,7 +283,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     window = static_cast<int64_t>(index) << p.page_shift < keys ? p.block_table[static_cast<int64_t>(b) * p.width + index] : -1;
   };
   auto begin_unit = [&]() {
-    head_src = p.cache + head * block_bytes;
+    head_src = p.cache + static_cast<uint64_t>(head) * block_bytes;
     load_window();
   };
   auto issue = [&](int stage) {
@@ -276,44 +302,29 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     good1 = good1 && rows > 16;
     if (lane == 0) infos[warp][stage] = make_int4(b, head, block, (tile << 3) | (good0 ? 1 : 0) | (good1 ? 2 : 0) | (tile == tiles - 1 ? 4 : 0));
     const int row = token & (page - 1);
-    const uint8_t* src0 = good0 ? head_src + page0 * page_bytes : p.cache;
-    const uint8_t* src1 = two_parts ? (good1 ? head_src + page1 * page_bytes : p.cache) : src0 + 16 * (kDim / 2);
-    const int64_t value_offset = p.kv_heads * block_bytes;
-    const uint8_t* code0 = src0 + row * (kDim / 2) + 16 * lane;
-    const uint8_t* code1 = src1 + (two_parts ? 0 : row * (kDim / 2)) + 16 * lane;
+    const uint8_t* src0 = head_src + static_cast<uint64_t>(static_cast<unsigned>(good0 ? page0 : 0)) * page_bytes + row * (kDim / 2);
+    const uint8_t* src1 = two_parts ? head_src + static_cast<uint64_t>(static_cast<unsigned>(good1 ? page1 : 0)) * page_bytes : src0 + 16 * (kDim / 2);
+    constexpr int kCopies = kRowPieces / 2, kPerCopy = 32 / kRowPieces;        // copies for 16 rows of codes, rows a copy covers
+    constexpr int kValues = Cfg::kCodeBytes + Cfg::kPairBytes;
     const uint32_t dst = lane_code + stage * Cfg::kStageBytes;
-    constexpr int kCopies = kRowPieces / 2;              // copy instructions for 16 rows of codes
     // the pairs: lanes 0..7 the keys', 8..15 the values', four tokens each
-    const int pair_token = 4 * (lane & 7);
-    const bool pair_second = pair_token >= 16;
-    const uint8_t* pair_src = (two_parts && pair_second ? src1 - 64 : src0 + 4 * row) + page * (kDim / 2) + 4 * pair_token +
-                              (lane & 8 ? value_offset : 0);
-    const uint32_t pair_dst = ring_base + stage * Cfg::kStageBytes + Cfg::kCodeBytes + 4 * pair_token +
-                              (lane & 8 ? Cfg::kCodeBytes + Cfg::kPairBytes : 0);
-    if (rows == kKv4Tile && good0 && good1) {
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        copy16(dst + 512 * i, code0 + 512 * i, 16);
-        copy16(dst + 512 * (kCopies + i), code1 + 512 * i, 16);
-        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * i, code0 + value_offset + 512 * i, 16);
-        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * (kCopies + i), code1 + value_offset + 512 * i, 16);
-      }
-      if (lane < 16) copy16(pair_dst, pair_src, 16);
+    const uint8_t* pair_src = (two_parts && pair_token >= 16 ? src1 - 64 : src0 + row * (4 - kDim / 2)) + pair_offset;
+    const uint32_t pair_at = pair_dst + stage * Cfg::kStageBytes;
+    if (rows >= kKv4Tile && good0 && good1) {
+      copy_rows<kCopies, 0>(dst, src0 + 16 * lane);
+      copy_rows<kCopies, 512 * kCopies>(dst, src1 + 16 * lane);
+      copy_rows<kCopies, kValues>(dst, src0 + value_lane);
+      copy_rows<kCopies, kValues + 512 * kCopies>(dst, src1 + value_lane);
+      if (lane < 16) copy16<0, 0>(pair_at, pair_src);
     } else {
       // rows behind the last key or on a page that cannot be followed are filled with zeros: scale 0, zero point 0
-#pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int r = lane_row + i * (32 / kRowPieces);
-        const int bytes0 = good0 && r < rows ? 16 : 0, bytes1 = good1 && r + 16 < rows ? 16 : 0;
-        copy16(dst + 512 * i, bytes0 ? code0 + 512 * i : p.cache, bytes0);
-        copy16(dst + 512 * (kCopies + i), bytes1 ? code1 + 512 * i : p.cache, bytes1);
-        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * i, bytes0 ? code0 + value_offset + 512 * i : p.cache, bytes0);
-        copy16(dst + Cfg::kCodeBytes + Cfg::kPairBytes + 512 * (kCopies + i), bytes1 ? code1 + value_offset + 512 * i : p.cache, bytes1);
-      }
-      if (lane < 16) {
-        const int bytes = (pair_second ? good1 : good0) ? 4 * max(0, min(4, rows - pair_token)) : 0;
-        copy16(pair_dst, bytes ? pair_src : p.cache, bytes);
-      }
+      // (their source is an address that is not read: a copy of no bytes)
+      const int rows0 = good0 ? rows : 0, rows1 = good1 ? rows - 16 : 0;
+      copy_rows<kCopies, 0, kPerCopy>(dst, src0 + 16 * lane, rows0, lane_row);
+      copy_rows<kCopies, 512 * kCopies, kPerCopy>(dst, src1 + 16 * lane, rows1, lane_row);
+      copy_rows<kCopies, kValues, kPerCopy>(dst, src0 + value_lane, rows0, lane_row);
+      copy_rows<kCopies, kValues + 512 * kCopies, kPerCopy>(dst, src1 + value_lane, rows1, lane_row);
+      if (lane < 16) copy16<0, 0>(pair_at, pair_src, 4 * max(0, min(4, pair_token >= 16 ? rows1 + 16 - pair_token : rows0 - pair_token)));
     }
     if (++tile == tiles) {                               // the next block of rows, head or sequence
       tile = 0;
