@@ -52,21 +52,24 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, bool b_transpose
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
-// Operand tiles are stored as segments of 64 components: rows of 128 bytes, swizzled. The same tile serves as keys
-// (K-major: components along K) and as values (components along N: `segment` is the distance between segments).
-__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr, uint32_t segment) {
-  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(segment >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// Operand tiles are stored as segments of 64 components: rows of 128 bytes, swizzled (the descriptor's upper word says
+// so). The same tile serves as keys (K-major: components along K) and as values (components along N: `segment` is the
+// distance between segments, in the lower word beside the address). A step of n bytes adds n / 16 to the lower word. The
+// issuing warp shares its scheduler with three busy ones, so an MMA must cost it few instructions: one addition a
+// descriptor.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr, uint32_t segment) { return ((smem_addr & 0x3FFFFu) >> 4) | ((segment >> 4) << 16); }
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
 }
-__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-               "r"(idesc), "r"(accumulate)
-               : "memory");
-}
-__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-               "r"(idesc), "r"(accumulate)
-               : "memory");
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
@@ -83,6 +86,12 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float kv4_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -131,7 +140,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
   constexpr int kSoftmaxGroups = kQTiles;
   constexpr uint32_t kOutputColumn = 256;
   extern __shared__ uint8_t dynamic_smem[];
-  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2], bar_done[2], bar_k[kStages], bar_k_free[kStages], bar_v[kStages], bar_v_free[kStages];
+  __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_done[2], bar_k[kStages], bar_k_free[kStages], bar_v[kStages], bar_v_free[kStages];
   __shared__ __align__(8) uint64_t bar_scale_k[kKv4ScaleSlots], bar_scale_v[kKv4ScaleSlots];
   __shared__ __align__(16) float scale_k[kKv4ScaleSlots][kKeys], scale_v[kKv4ScaleSlots][kKeys];
   __shared__ uint32_t hidden[kKv4MarkSlots][kKeys / 32];   // keys of the tile on a page that could not be followed
@@ -150,7 +159,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       mbar_init(smem_u32(&bar_q), 128 * kQTiles);
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&bar_s[i]), 1);
-        mbar_init(smem_u32(&bar_p[i]), 128);
+        mbar_init(smem_u32(&bar_p[i][0]), 128);
+        mbar_init(smem_u32(&bar_p[i][1]), 128);
         mbar_init(smem_u32(&bar_done[i]), 1);
       }
       for (int i = 0; i < kStages; ++i) {
@@ -212,17 +222,26 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         // the tile's queries, in the unpacked codes' order
         constexpr int kPieces = kDim / 8;
         uint8_t* const tile = q_smem + t * Cfg::kQBytes;
-        for (int i = row_in_tile; i < 128 * kPieces; i += 128) {
-          const int r = i / kPieces, piece = i % kPieces, q_row = first_row + 128 * t + r;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (q_row < all_rows) {
-            const int token = p.group.quotient(q_row);
-            w = *reinterpret_cast<const uint4*>(p.q + (seq.start + token) * p.q_stride +
-                                                static_cast<int64_t>(head * group + q_row - token * group) * kDim + 8 * piece);
+#pragma unroll 1
+        for (int base = row_in_tile; base < 128 * kPieces; base += 8 * 128) {
+          uint4 w[8];                                    // eight loads in flight
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int i = base + 128 * n, q_row = first_row + 128 * t + i / kPieces;
+            w[n] = make_uint4(0, 0, 0, 0);
+            if (q_row < all_rows) {
+              const int token = p.group.quotient(q_row);
+              w[n] = *reinterpret_cast<const uint4*>(p.q + (seq.start + token) * p.q_stride +
+                                                     static_cast<int64_t>(head * group + q_row - token * group) * kDim + 8 * (i % kPieces));
+            }
           }
-          const uint4 turned = make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
-                                          __byte_perm(w.y, w.w, 0x7632));
-          *reinterpret_cast<uint4*>(tile + (piece / 8) * (128 * 128) + r * 128 + ((piece % 8) ^ (r & 7)) * 16) = turned;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int i = base + 128 * n, r = i / kPieces, piece = i % kPieces;
+            *reinterpret_cast<uint4*>(tile + (piece / 8) * (128 * 128) + r * 128 + ((piece % 8) ^ (r & 7)) * 16) =
+                make_uint4(__byte_perm(w[n].x, w[n].z, 0x5410), __byte_perm(w[n].x, w[n].z, 0x7632), __byte_perm(w[n].y, w[n].w, 0x5410),
+                           __byte_perm(w[n].y, w[n].w, 0x7632));
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bar_q));
@@ -276,7 +295,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
 #pragma unroll
         for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[c][i]));
+          for (int i = 0; i < 32; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
         const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
         if (__any_sync(0xffffffffu, most > m + 8.f)) {
           const float next = fmaxf(m, most);
@@ -326,10 +345,10 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
             packed[i / 2 + 1] = pack2(y.x, y.y);
           }
           tmem_st_32x32(scores + 32 * h, packed);
+          tmem_st_wait();
+          tcgen05_fence_before();
+          mbar_arrive(smem_u32(&bar_p[buffer][h]));      // the product may begin on the first half of the keys
         }
-        tmem_st_wait();
-        tcgen05_fence_before();
-        mbar_arrive(smem_u32(&bar_p[buffer]));
       }
       // ---- output
       if (fine && tiles > 0) fine = warp_wait(&bar_done[t], 0, &abort_flag);
@@ -392,7 +411,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       const int lane_row = (kDim == 64 ? 16 * (warp % 4) + 8 * (octet / 2) : 8 * (warp % 4)) + lane % 8;
       const int lane_piece = kDim == 64 ? octet % 2 : octet;
       const int page = 1 << p.page_shift;
-      const int64_t block_bytes = kv4_block_bytes(page, kDim);
+      const unsigned block_bytes = page * (kDim / 2 + 4), page_bytes = block_bytes * kKv4Side * p.kv_heads;   // at most 70 MB
+      const uint8_t* const head_src = p.cache + static_cast<uint64_t>(head) * block_bytes;
       const int32_t* const table = p.block_table + static_cast<int64_t>(b) * p.width;
       // page numbers of the keys ahead: 32 in the lanes and the next 32 behind them
       int window_first = begin * kKeys >> p.page_shift;
@@ -402,9 +422,12 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       };
       int window = load_window(window_first), window_next = load_window(window_first + 32);
       uint4 codes[kPasses][kLoads];
-      uint32_t pairs[kPasses];                           // bit 31 of a pair's scale marks a page that cannot be followed
+      uint32_t pairs[kPasses];                           // (nothing may touch what is loaded before the next half-step)
+      uint32_t marks = 0, live = 0;                      // passes whose key lies on a page that cannot be followed, whose key is there
       auto load = [&](int step) {
         const int tile = begin + step / kSteps, side = kSteps == 2 ? step & 1 : side_first;
+        const uint8_t* const side_src = head_src + side * p.kv_heads * block_bytes;
+        marks = live = 0;
         while ((((tile + 1) * kKeys - 1) >> p.page_shift) - window_first >= 32 + 32) {
           window_first += 32;
           window = window_next;
@@ -415,15 +438,15 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           const int key = tile * kKeys + kPassRows * i + lane_row;
           const int index = (key >> p.page_shift) - window_first;
           const int low = __shfl_sync(0xffffffffu, window, index & 31), high = __shfl_sync(0xffffffffu, window_next, index & 31);
-          const int id = index < 32 ? low : high;
-          const bool wanted = key < keys, good = wanted && static_cast<unsigned>(id) < static_cast<unsigned>(p.pages);
-#pragma unroll
-          for (int n = 0; n < kLoads; ++n) codes[i][n] = make_uint4(0, 0, 0, 0);
-          pairs[i] = wanted ? 0x8000u : 0u;
-          if (good) {
-            const uint8_t* src = p.cache + ((static_cast<int64_t>(id) * kKv4Side + side) * p.kv_heads + head) * block_bytes;
-            const int at = key & (page - 1);
-            pairs[i] = __ldcg(reinterpret_cast<const unsigned*>(src + page * (kDim / 2) + 4 * at)) & 0xffff7fffu;
+          const unsigned id = index < 32 ? low : high;
+          const bool wanted = key < keys, good = wanted && id < static_cast<unsigned>(p.pages);
+          marks |= wanted && !good ? 1u << i : 0u;
+          live |= good ? 1u << i : 0u;
+          // a key that is not there reads the cache's first page instead and is made zero when it is used
+          const uint8_t* src = side_src + static_cast<uint64_t>(good ? id : 0u) * page_bytes;
+          const int at = key & (page - 1);
+          if (p.pages > 0) {
+            pairs[i] = __ldcg(reinterpret_cast<const unsigned*>(src + page * (kDim / 2) + 4 * at));
 #pragma unroll
             for (int n = 0; n < kLoads; ++n)
               codes[i][n] = __ldcg(reinterpret_cast<const uint4*>(src + at * (kDim / 2) + 16 * (lane_piece + 4 * n)));
@@ -440,6 +463,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         uint64_t* const empty = side ? bar_v_free : bar_k_free;
         uint4 now[kPasses][kLoads];
         uint32_t now_pairs[kPasses];
+        const uint32_t now_marks = marks, now_live = live;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
           now_pairs[i] = pairs[i];
@@ -449,19 +473,24 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         if (step + 1 < steps) load(step + 1);
         if (j >= kStages) fine = warp_wait(&empty[stage], (j / kStages - 1) & 1, &abort_flag);
         if (!fine) break;
+        if (now_live != (1u << kPasses) - 1) {
+#pragma unroll
+          for (int i = 0; i < kPasses; ++i) {
+            if (now_live >> i & 1) continue;
+            now_pairs[i] = 0;
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) now[i][n] = make_uint4(0, 0, 0, 0);
+          }
+        }
         uint8_t* const tile = (side ? v_smem : k_smem) + stage * Cfg::kTileBytes;
-        bool bad = false;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
           const int row = kPassRows * i + lane_row;
-          const bool marked = now_pairs[i] & 0x8000u;
           const float zero = 128.f + bf16_hi(now_pairs[i]);
           const uint32_t zeros = pack2(zero, zero);
           if (lane_piece == 0) {
-            if (side) scale_v[slot][row] = marked ? 0.f : bf16_lo(now_pairs[i]);
-            else scale_k[slot][row] = marked ? 0.f : bf16_lo(now_pairs[i]);
+            (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]);
           }
-          bad |= marked;
 #pragma unroll
           for (int n = 0; n < kLoads; ++n) {
             const int piece = lane_piece + 4 * n;
@@ -485,13 +514,13 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
             if (lane < kKeys / 32) hidden[clear][lane] = 0;
             if (lane == 0) any_hidden[clear] = 0;
           }
-          if (bad) {
+          if (now_marks) {
             any_hidden[j % kKv4MarkSlots] = 1;
             atomicOr(&g_ci8_status, kStatusBadIndex);
 #pragma unroll
             for (int i = 0; i < kPasses; ++i) {
               const int row = kPassRows * i + lane_row;
-              if (now_pairs[i] & 0x8000u) atomicOr(&hidden[j % kKv4MarkSlots][row / 32], 1u << (row % 32));
+              if (now_marks >> i & 1) atomicOr(&hidden[j % kKv4MarkSlots][row / 32], 1u << (row % 32));
             }
           }
           mbar_arrive(smem_u32(&bar_scale_k[slot]));
@@ -506,27 +535,33 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       if (warp == 12 && tiles > 0) {
         // ================================================================ MMA issue
         constexpr uint32_t kIdescS = idesc_bf16(128, kKeys, false), kIdescO = idesc_bf16(128, kDim, true);
-        const uint32_t q_at = smem_u32(q_smem), k_at = smem_u32(k_smem), v_at = smem_u32(v_smem);
+        const uint32_t q_desc = desc_low(smem_u32(q_smem), 16), k_desc = desc_low(smem_u32(k_smem), 16);
+        const uint32_t v_desc = desc_low(smem_u32(v_smem), kKeys * 128);
+        constexpr uint32_t kTileStep = Cfg::kTileBytes / 16, kQStep = Cfg::kQBytes / 16;
         auto scores = [&](int t, int buffer, int stage) {
+          const uint32_t d = tmem + 128 * buffer, a = q_desc + t * kQStep, b = k_desc + stage * kTileStep;
           if (elect_one()) {
 #pragma unroll
             for (int s = 0; s < kSegments; ++s)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_bf16_ss(tmem + 128 * buffer, smem_desc_sw128(q_at + t * Cfg::kQBytes + s * (128 * 128)) + 2 * k,
-                            smem_desc_sw128(k_at + stage * Cfg::kTileBytes + s * (kKeys * 128)) + 2 * k, kIdescS, s + k > 0);
+              for (int k = 0; k < 4; ++k) mma_bf16_ss(d, a + s * (128 * 128 / 16) + 2 * k, b + s * (kKeys * 128 / 16) + 2 * k, kIdescS, s + k > 0);
             mma_commit(smem_u32(&bar_s[buffer]));
           }
           __syncwarp();
         };
-        auto outputs = [&](int t, int buffer, int stage, bool accumulate) {
-          if (elect_one()) {
+        auto outputs = [&](int t, int buffer, int stage, int parity, bool accumulate) {   // waits for the weights, 64 keys at a time
+          for (int h = 0; h < kKeys / 64; ++h) {
+            if (!warp_wait(&bar_p[buffer][h], parity, &abort_flag)) return false;
+            tcgen05_fence_after();
+            const uint32_t d = tmem + kOutputColumn + t * kDim, a = tmem + 128 * buffer + 32 * h, b = v_desc + stage * kTileStep + h * (8192 / 16);
+            if (elect_one()) {
+              mma_bf16_ts(d, a, b, kIdescO, accumulate || h > 0);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              mma_bf16_ts(tmem + kOutputColumn + t * kDim, tmem + 128 * buffer + 8 * k,
-                          smem_desc_sw128_mn(v_at + stage * Cfg::kTileBytes + k * 2048, kKeys * 128), kIdescO, accumulate || k > 0);
+              for (int k = 1; k < 4; ++k) mma_bf16_ts(d, a + 8 * k, b + k * (2048 / 16), kIdescO, 1);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          return true;
         };
         auto commit = [&](uint64_t* bar) {
           if (elect_one()) mma_commit(smem_u32(bar));
@@ -540,10 +575,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
               if (j > 0) {
                 const int stage = (j - 1) % kStages;
                 if (t == 0) fine = warp_wait(&bar_v[stage], (j - 1) / kStages & 1, &abort_flag);
-                fine = fine && warp_wait(&bar_p[t], (j - 1) & 1, &abort_flag);
+                fine = fine && outputs(t, t, stage, (j - 1) & 1, j > 1);
                 if (!fine) break;
-                tcgen05_fence_after();
-                outputs(t, t, stage, j > 1);
                 if (t == 1) commit(&bar_v_free[stage]);
                 if (j == tiles) commit(&bar_done[t]);
               }
@@ -571,11 +604,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
             }
             if (j > 0) {
               const int stage = (j - 1) % kStages, buffer = (j - 1) & 1;
-              fine = warp_wait(&bar_v[stage], (j - 1) / kStages & 1, &abort_flag) &&
-                     warp_wait(&bar_p[buffer], (j - 1) >> 1 & 1, &abort_flag);
+              fine = warp_wait(&bar_v[stage], (j - 1) / kStages & 1, &abort_flag) && outputs(0, buffer, stage, (j - 1) >> 1 & 1, j > 1);
               if (!fine) break;
-              tcgen05_fence_after();
-              outputs(0, buffer, stage, j > 1);
               commit(&bar_v_free[stage]);
               commit(&bar_done[j == tiles ? 0 : 1]);
             }
