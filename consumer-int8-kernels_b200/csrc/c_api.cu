@@ -840,24 +840,39 @@ bool kv4_rotation(const float* cos_sin, int table_rows, int rotary, const int64_
          axes > 0 && axes <= 4 && aligned(axis_of, 4) && (axis_of || axes == 1);
 }
 
-// Heads of a token go to one warp while there are tokens enough to fill the GPU with four batches of loads per
-// warp, and are cut into single batches otherwise (a generated token: 28 heads of 256 components on 28 warps
-// instead of 1).
+// How many warps share the heads of one token, `steps` loads each at most: enough warps to fill the GPU a few times over
+// where the tokens are few (a generated token: 28 heads of 256 components on 28 warps), whole batches of loads otherwise.
+int kv4_chunks(int tokens, long long steps, long long batch) {
+  const long long busy = static_cast<long long>(sm_count()) * 128;
+  long long chunks = (busy + tokens - 1) / tokens;
+  const long long batches = (steps + batch - 1) / batch;
+  if (tokens >= sm_count() * 8 && chunks > batches) chunks = batches;
+  return static_cast<int>(chunks < steps ? chunks : steps);
+}
 template <int kDim, bool kNorm, bool kAppend>
 int launch_kv4_rows(Kv4RowParams p, ci8_stream_t stream) {
   const int per_step = 32 / (kDim / 8);
   const int heads = (p.q ? p.q_heads : 0) + p.kv_heads * (kAppend ? 2 : 1);
   const long long steps = (heads + per_step - 1) / per_step;
-  const long long busy = static_cast<long long>(sm_count()) * 32;
-  long long chunks = (busy + p.tokens - 1) / p.tokens;
-  if (chunks > steps) chunks = steps;
-  const long long four = (steps + 3) / 4;
-  if (chunks < four) chunks = four;
+  const long long chunks = kv4_chunks(p.tokens, steps, 4);
+  const long long per_chunk = ((steps + chunks - 1) / chunks) * per_step;   // whole steps
+  p.chunks = static_cast<int>((heads + per_chunk - 1) / per_chunk);
+  const long long warps = static_cast<long long>(p.tokens) * p.chunks;
+  const int per_cta = warps < 8 * sm_count() ? 1 : 8;
+  if (warps / per_cta >= 0x7fffffffll) return kInvalid;
+  return launch_pdl(kv4_rows_kernel<kDim, kNorm, kAppend>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
+}
+template <int kDim>
+int launch_kv4_read(Kv4ReadParams p, ci8_stream_t stream) {
+  const int per_step = 32 / (kDim / 8), heads = 2 * p.kv_heads;
+  const long long steps = (heads + per_step - 1) / per_step;
+  const long long chunks = kv4_chunks(p.tokens, steps, 8);
   const long long per_chunk = ((steps + chunks - 1) / chunks) * per_step;
   p.chunks = static_cast<int>((heads + per_chunk - 1) / per_chunk);
   const long long warps = static_cast<long long>(p.tokens) * p.chunks;
-  const int per_cta = warps < 4 * sm_count() ? 1 : 8;
-  return launch_pdl(kv4_rows_kernel<kDim, kNorm, kAppend>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
+  const int per_cta = warps < 8 * sm_count() ? 1 : 8;
+  if (warps / per_cta >= 0x7fffffffll) return kInvalid;
+  return launch_pdl(kv4_read_kernel<kDim>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
 }
 template <bool kNorm, bool kAppend>
 int launch_kv4_rows(const Kv4RowParams& p, int dim, ci8_stream_t stream) {
@@ -1369,15 +1384,9 @@ int ci8_kv4_read(const void* cache, const int64_t* slots, void* k, void* v, int 
   Kv4ReadParams p = {};
   p.cache = static_cast<const uint8_t*>(cache); p.slots = slots;
   p.k = static_cast<uint16_t*>(k); p.v = static_cast<uint16_t*>(v);
-  p.capacity = static_cast<int64_t>(pages) << shift; p.rows = static_cast<int64_t>(tokens) * 2 * kv_heads;
-  p.kv_heads = kv_heads; p.page_shift = shift;
-  const int64_t per_cta = 256 / (dim / 8);
-  int64_t grid = (p.rows + per_cta - 1) / per_cta;
-  const int64_t most = static_cast<int64_t>(sm_count()) * 8;
-  if (grid > most) grid = most;
-  return dim == 64 ? launch_pdl(kv4_read_kernel<64>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p)
-         : dim == 128 ? launch_pdl(kv4_read_kernel<128>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p)
-                      : launch_pdl(kv4_read_kernel<256>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p);
+  p.capacity = static_cast<int64_t>(pages) << shift;
+  p.tokens = tokens; p.kv_heads = kv_heads; p.page_shift = shift;
+  return dim == 64 ? launch_kv4_read<64>(p, stream) : dim == 128 ? launch_kv4_read<128>(p, stream) : launch_kv4_read<256>(p, stream);
 }
 
 long long ci8_kv4_workspace_bytes(void) { return kKv4WorkspaceBytes; }

@@ -44,49 +44,57 @@ struct Kv4RowParams {
   float eps, weight_offset;
 };
 
-// Scale and zero point of one head whose smallest component is low <= 0 and largest high >= 0. The scale
-// is rounded to BF16 before the codes are taken, so that the codes are the best ones for the scale that is
-// kept; the zero point is a whole number, so the value 0 is kept exactly.
+// Scale and zero point of one head whose smallest component is low <= 0 and largest high >= 0. The scale is rounded to
+// BF16 before the codes are taken, so that the codes are the best ones for the scale that is kept; the zero point is a
+// whole number, so the value 0 is kept exactly.
 struct Kv4Code {
-  float scale, inverse;
-  int zero;
+  float scale, inverse, zero;   // inverse: an approximation, for the short path below
 };
+__device__ __forceinline__ float approximate_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ Kv4Code kv4_code_of(float low, float high) {
   Kv4Code c;
   const float step = __fdiv_rn(__fsub_rn(high, low), 15.f);
   c.scale = fmaxf(__bfloat162float(__float2bfloat16_rn(step)), __bfloat162float(__float2bfloat16_rn(1e-20f)));
-  c.inverse = __frcp_rn(c.scale);
-  c.zero = min(15, __float2int_rn(__fdiv_rn(-low, c.scale)));
+  c.inverse = approximate_reciprocal(c.scale);
+  float rounded = __fsub_rn(__fmaf_rn(-low, c.inverse, kRoundMagic), kRoundMagic);
+  if (!away_from_tie(-low, c.inverse)) rounded = rintf(__fdiv_rn(-low, c.scale));
+  c.zero = fminf(15.f, rounded);
   return c;
 }
 
-// Eight components -> eight codes in one word, clamp(rint(x / scale) + zero, 0, 15) with the IEEE quotient:
-// the quantizer's short path (a product with the reciprocal, proven equal away from ties) and its repair.
-__device__ __forceinline__ uint32_t kv4_encode8(const float (&x)[8], const Kv4Code& code) {
+// Eight components -> eight codes in one word, clamp(rint(x / scale) + zero, 0, 15) with the IEEE quotient: the
+// quantizer's short path (a product with the reciprocal, equal away from ties: with a reciprocal that is off by one unit
+// in the last place the product is off by less than 17 * 2^-22, well inside the guard band) and its repair. The zero
+// point goes into the constant that rounds (rint(q) + zero = rint(q + zero) but for ties, which are repaired), and the
+// codes are put together as a sum of t * 16^j, whose constant part is taken off at the end.
+__device__ __forceinline__ uint32_t kv4_encode8(const float2 (&x)[4], const Kv4Code& code) {
+  const float2 inverse = make_float2(code.inverse, code.inverse), magic = make_float2(kRoundMagic, kRoundMagic);
+  const float2 offset = make_float2(code.zero, code.zero);
   float worst = 0.f;
-  int t[8];
+  float t[8];
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const float2 shifted = quantize_fast2(make_float2(x[j], x[j + 1]), make_float2(code.inverse, code.inverse), worst);
-    t[j] = __float_as_int(shifted.x) - __float_as_int(kRoundMagic);
-    t[j + 1] = __float_as_int(shifted.y) - __float_as_int(kRoundMagic);
+  for (int j = 0; j < 4; ++j) {
+    const float2 shifted = quantize_fast2(x[j], inverse, worst);
+    const float2 moved = __fadd2_rn(shifted, offset);    // exact
+    t[2 * j] = moved.x;
+    t[2 * j + 1] = moved.y;
   }
   if (!(fabsf(worst) < kTieGuard)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (!away_from_tie(x[j], code.inverse)) t[j] = __float2int_rn(__fdiv_rn(x[j], code.scale));
+    for (int j = 0; j < 8; ++j) {
+      const float v = j % 2 ? x[j / 2].y : x[j / 2].x;
+      if (!away_from_tie(v, code.inverse)) t[j] = kRoundMagic + (rintf(__fdiv_rn(v, code.scale)) + code.zero);
+    }
   }
   uint32_t word = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) word |= static_cast<uint32_t>(min(15, max(0, t[j] + code.zero))) << (4 * j);
-  return word;
-}
-
-template <int kLanes>
-__device__ __forceinline__ float head_sum(float v) {
-#pragma unroll
-  for (int d = kLanes / 2; d; d /= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
+  for (int j = 0; j < 8; ++j)
+    word += __float_as_uint(fminf(fmaxf(t[j], kRoundMagic), kRoundMagic + 15.f)) * (1u << (4 * j));
+  return word - 0x4B400000u * 0x11111111u;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
@@ -100,16 +108,37 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
 }
+__device__ __forceinline__ float2 unpack2(uint32_t w) { return make_float2(bf16_lo(w), bf16_hi(w)); }
+// x * cosine + partner * sine with every product and the sum rounded on its own. (The packed intrinsics are no barrier to
+// contraction; single products and sums with a rounding mode are.)
+__device__ __forceinline__ float2 turn2(float2 x, float2 cosine, float2 partner, float2 sine) {
+  return make_float2(__fadd_rn(__fmul_rn(x.x, cosine.x), __fmul_rn(partner.x, sine.x)),
+                     __fadd_rn(__fmul_rn(x.y, cosine.y), __fmul_rn(partner.y, sine.y)));
+}
+// Minimum and maximum that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-// One warp takes a piece of one token's heads (queries, keys and, when appending, values, in that order): the
-// token's angles stay in registers and up to kBatch heads per lane group are loaded before the first is used.
-// Norm and rotation are FP32; products and sums of the rotation are rounded one by one (no FMA), so that what is
-// encoded does not depend on how a compiler contracts them. Bound by memory: 4 bytes per component of the norm,
-// 2 read + dim / 2 + 4 bytes per head written for what is appended.
+// One warp takes a piece of one token's heads (queries, keys and, when appending, values, in that order): the token's
+// angles and the norm's weights stay in registers, and up to kBatch heads per lane group are loaded before the first is
+// used. A lane holds two runs of four components. Turning components (i, i + rotary / 2), it holds both of a pair: runs
+// 4 l and rotary / 2 + 4 l, so the rotation needs no exchange between lanes; otherwise its runs are neighbours. FP32
+// throughout, two components to an instruction; products and sums of the rotation are rounded one by one (no FMA), so
+// that what is encoded does not depend on how a compiler contracts them. Bound by memory: 4 bytes per component of the
+// norm, 2 read and dim / 2 + 4 bytes per head written for what is appended.
 template <int kDim, bool kNorm, bool kAppend>
 __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4RowParams p) {
   constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 4;
   pdl_wait();
+  pdl_launch_dependents();
   const int warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
   const int token = warp / p.chunks, chunk = warp % p.chunks;
   if (token >= p.tokens) return;      // whole warps
@@ -118,161 +147,170 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4RowParams p) {
   const int heads = q_heads + p.kv_heads * (kAppend ? 2 : 1);
   const int per_chunk = (heads + p.chunks - 1) / p.chunks;
   const int first = chunk * per_chunk, end = min(heads, first + per_chunk);
+  const bool turns = l < p.rotary / 8;                  // rotary is 0 without a table
+  const int run0 = turns && !p.adjacent ? 4 * l : 8 * l, run1 = turns && !p.adjacent ? p.rotary / 2 + 4 * l : 8 * l + 4;
 
-  // The token's angles: cosine and sine of each of this lane's components (adjacent pairs: of its four pairs).
-  float cosine[8], sine[8];
+  const uint16_t* const q_src = p.q ? p.q + token * p.q_stride : nullptr;
+  const uint16_t* const k_src = p.k + token * p.k_stride;
+  const uint16_t* const v_src = kAppend ? p.v + token * p.v_stride : nullptr;
+  uint2 raw[kBatch][2];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = base + i * kHeadsPerStep + sub;
+      raw[i][0] = raw[i][1] = make_uint2(0, 0);
+      if (h < end) {
+        const uint16_t* src = h < q_heads ? q_src + h * kDim
+                              : (!kAppend || h < q_heads + p.kv_heads) ? k_src + (h - q_heads) * kDim : v_src + (h - q_heads - p.kv_heads) * kDim;
+        raw[i][0] = *reinterpret_cast<const uint2*>(src + run0);
+        raw[i][1] = *reinterpret_cast<const uint2*>(src + run1);
+      }
+    }
+  };
+  load(first);
+
+  // The token's angles: y[i] = x[i] * cosine[i] + partner[i] * sine[i] over pairs of components.
+  float2 cosine[4], sine[4];
   bool bad = false;
-  const int half_lanes = p.rotary / 16;                 // lanes that hold the first components of the pairs
-  const bool turns = p.cos_sin != nullptr && l < p.rotary / 8;
   if (p.cos_sin) {
     for (int a = 0; a < p.axes; ++a) {
       const int64_t place = p.positions[static_cast<int64_t>(a) * p.tokens + token];
       bad |= place < 0 || place >= p.table_rows;
     }
-    const int pairs = p.rotary / 2;
-    const int count = p.adjacent ? 4 : 8;
-    const int f0 = p.adjacent ? 4 * l : 8 * (l < half_lanes ? l : l - half_lanes);
+    float c[4] = {}, s[4] = {};
+    const int f = 4 * l, pairs = p.rotary / 2;           // this lane's four pairs, either way of pairing
     if (turns && !bad) {
       if (!p.axis_of) {
-        const float* row = p.cos_sin + p.positions[token] * p.rotary;
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          if (j < count) {
-            const float4 c = *reinterpret_cast<const float4*>(row + f0 + j);
-            const float4 s = *reinterpret_cast<const float4*>(row + pairs + f0 + j);
-            cosine[j] = c.x; cosine[j + 1] = c.y; cosine[j + 2] = c.z; cosine[j + 3] = c.w;
-            sine[j] = s.x; sine[j + 1] = s.y; sine[j + 2] = s.z; sine[j + 3] = s.w;
-          }
-        }
+        const float* row = p.cos_sin + p.positions[token] * p.rotary + f;
+        const float4 cs = *reinterpret_cast<const float4*>(row), sn = *reinterpret_cast<const float4*>(row + pairs);
+        c[0] = cs.x; c[1] = cs.y; c[2] = cs.z; c[3] = cs.w;
+        s[0] = sn.x; s[1] = sn.y; s[2] = sn.z; s[3] = sn.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j < count) {
-            const int axis = p.axis_of[f0 + j];
-            if (axis < 0 || axis >= p.axes) {
-              bad = true;
-            } else {
-              const float* row = p.cos_sin + p.positions[static_cast<int64_t>(axis) * p.tokens + token] * p.rotary;
-              cosine[j] = row[f0 + j];
-              sine[j] = row[pairs + f0 + j];
-            }
+        for (int j = 0; j < 4; ++j) {
+          const int axis = p.axis_of[f + j];
+          if (axis < 0 || axis >= p.axes) {
+            bad = true;
+          } else {
+            const float* row = p.cos_sin + p.positions[static_cast<int64_t>(axis) * p.tokens + token] * p.rotary + f + j;
+            c[j] = row[0];
+            s[j] = row[pairs];
           }
         }
       }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = j % 2 * 2;                           // not adjacent: components 0..3 with 4..7
+      cosine[j] = p.adjacent ? make_float2(c[j], c[j]) : make_float2(c[e], c[e + 1]);
+      sine[j] = p.adjacent ? make_float2(-s[j], s[j]) : j < 2 ? make_float2(-s[e], -s[e + 1]) : make_float2(s[e], s[e + 1]);
     }
   }
   bad = __any_sync(0xffffffffu, bad);
-
-  int64_t slot = -1;
-  if constexpr (kAppend) {
-    slot = p.slots[token];
-    if (slot >= p.capacity) {
-      slot = -1;
-      if (lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
-    }
-    if (bad) slot = -1;
-  }
   if (bad && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
 
-  for (int base = first; base < end; base += kBatch * kHeadsPerStep) {
-    uint4 raw[kBatch];
+  float2 q_weight[4], k_weight[4];
+  if constexpr (kNorm) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int h = base + i * kHeadsPerStep + sub;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (h < end) {
-        const uint16_t* src = h < q_heads ? p.q + token * p.q_stride + static_cast<int64_t>(h) * kDim
-                              : (!kAppend || h < q_heads + p.kv_heads)
-                                  ? p.k + token * p.k_stride + static_cast<int64_t>(h - q_heads) * kDim
-                                  : p.v + token * p.v_stride + static_cast<int64_t>(h - q_heads - p.kv_heads) * kDim;
-        raw[i] = *reinterpret_cast<const uint4*>(src + 8 * l);
+    for (int side = 0; side < 2; ++side) {
+      const uint16_t* weight = side ? p.k_weight : p.q_weight;
+      float2(&to)[4] = side ? k_weight : q_weight;
+      if (weight) {
+        const uint2 a = *reinterpret_cast<const uint2*>(weight + run0), b = *reinterpret_cast<const uint2*>(weight + run1);
+        const float2 offset = make_float2(p.weight_offset, p.weight_offset);
+        to[0] = __fadd2_rn(unpack2(a.x), offset);
+        to[1] = __fadd2_rn(unpack2(a.y), offset);
+        to[2] = __fadd2_rn(unpack2(b.x), offset);
+        to[3] = __fadd2_rn(unpack2(b.y), offset);
       }
     }
+  }
+
+  uint8_t* slot_page = nullptr;                          // the slot's page, null: not stored
+  int slot_row = 0;
+  const int page = 1 << p.page_shift;
+  const unsigned block_bytes = page * (kDim / 2 + 4);    // at most 32 KB
+  if constexpr (kAppend) {
+    const int64_t slot = p.slots[token];
+    if (slot >= p.capacity && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
+    if (slot >= 0 && slot < p.capacity && !bad) {
+      slot_page = p.cache + (slot >> p.page_shift) * kKv4Side * p.kv_heads * static_cast<int64_t>(block_bytes);
+      slot_row = static_cast<int>(slot & (page - 1));
+    }
+  }
+
+  for (int base = first; base < end; base += kBatch * kHeadsPerStep) {
+    if (base > first) load(base);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (base + i * kHeadsPerStep >= end) break;       // the same for the whole warp
+      if (base + i * kHeadsPerStep >= end) break;        // the same for the whole warp
       const int h = base + i * kHeadsPerStep + sub;
-      const bool is_q = h < q_heads, is_v = kAppend && h >= q_heads + p.kv_heads;
-      float x[8];
-      unpack8(raw[i], x);
+      const bool is_q = h < q_heads, is_v = kAppend && h >= q_heads + p.kv_heads, real = h < end;
+      float2 x[4] = {unpack2(raw[i][0].x), unpack2(raw[i][0].y), unpack2(raw[i][1].x), unpack2(raw[i][1].y)};
       if constexpr (kNorm) {
-        float squares = 0.f;
+        float2 squares = __fmul2_rn(x[0], x[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) squares = fmaf(x[j], x[j], squares);
-        const float scale = rsqrtf(head_sum<kLanes>(squares) * (1.f / kDim) + p.eps);
-        const uint16_t* weight = is_q ? p.q_weight : p.k_weight;
-        if (weight) {
-          float w[8];
-          unpack8(*reinterpret_cast<const uint4*>(weight + 8 * l), w);
+        for (int j = 1; j < 4; ++j) squares = __ffma2_rn(x[j], x[j], squares);
+        float sum = squares.x + squares.y;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = x[j] * scale * (w[j] + p.weight_offset);
+        for (int d = kLanes / 2; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float unit = rsqrtf(sum * (1.f / kDim) + p.eps);
+        if (is_q ? p.q_weight : p.k_weight) {
+          const float2 unit2 = make_float2(unit, unit);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = __fmul2_rn(__fmul2_rn(x[j], unit2), is_q ? q_weight[j] : k_weight[j]);
         }
       }
-      if (p.cos_sin) {
-        float y[8];
-        if (p.adjacent) {
+      if (turns && !is_v) {
+        float2 partner[4];
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            y[j] = __fsub_rn(__fmul_rn(x[j], cosine[j / 2]), __fmul_rn(x[j + 1], sine[j / 2]));
-            y[j + 1] = __fadd_rn(__fmul_rn(x[j + 1], cosine[j / 2]), __fmul_rn(x[j], sine[j / 2]));
-          }
-        } else {
-          const int partner = sub * kLanes + (turns ? (l < half_lanes ? l + half_lanes : l - half_lanes) : l);
+        for (int j = 0; j < 4; ++j) partner[j] = p.adjacent ? make_float2(x[j].y, x[j].x) : x[j ^ 2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float other = __shfl_sync(0xffffffffu, x[j], partner);
-            const float kept = __fmul_rn(x[j], cosine[j]), mixed = __fmul_rn(other, sine[j]);
-            y[j] = l < half_lanes ? __fsub_rn(kept, mixed) : __fadd_rn(kept, mixed);
-          }
-        }
-        if (turns && !is_v) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = y[j];
-        }
+        for (int j = 0; j < 4; ++j) x[j] = turn2(x[j], cosine[j], partner[j], sine[j]);
       }
-      const bool real = h < end;
-      if (!kAppend || is_q) {
-        if (real) {
-          uint4 w = pack8(x);
-          if (bad) w = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);   // a position outside the table: NaN
-          uint16_t* dst = is_q ? p.q_out + token * p.q_out_stride + static_cast<int64_t>(h) * kDim
-                               : p.k_out + token * p.k_out_stride + static_cast<int64_t>(h - q_heads) * kDim;
-          *reinterpret_cast<uint4*>(dst + 8 * l) = w;
-        }
+      if ((!kAppend || is_q) && real) {
+        uint2 a = make_uint2(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y)), b = make_uint2(pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y));
+        if (bad) a = b = make_uint2(0x7fff7fffu, 0x7fff7fffu);   // a position outside the table: NaN
+        uint16_t* dst = is_q ? p.q_out + token * p.q_out_stride + h * kDim : p.k_out + token * p.k_out_stride + (h - q_heads) * kDim;
+        *reinterpret_cast<uint2*>(dst + run0) = a;
+        *reinterpret_cast<uint2*>(dst + run1) = b;
       }
       if constexpr (kAppend) {
-        if (slot < 0 || base + i * kHeadsPerStep + kHeadsPerStep <= q_heads) continue;   // whole warps: nothing to encode here
-        float low = 0.f, high = 0.f, worst = 0.f;
+        if (!slot_page || base + (i + 1) * kHeadsPerStep <= q_heads) continue;   // whole warps: nothing to encode here
+        float low = 0.f, high = 0.f;
+        auto range = [&]() {
+          low = high = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) worst = max_abs_keep_nan(worst, x[j]);
-        if (!(fabsf(worst) < 8.5e37f)) {
+          for (int j = 0; j < 4; ++j) {
+            low = min_nan(low, min_nan(x[j].x, x[j].y));
+            high = max_nan(high, max_nan(x[j].x, x[j].y));
+          }
+#pragma unroll
+          for (int d = kLanes / 2; d; d /= 2) {
+            low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
+            high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
+          }
+        };
+        range();
+        if (__any_sync(0xffffffffu, !(low >= -8.5e37f && high <= 8.5e37f))) {
           // NaN counts as 0 and infinities as the largest value whose range still fits FP32, so that one such
           // component cannot spoil the scale and with it the whole head
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = x[j] != x[j] ? 0.f : fminf(fmaxf(x[j], -8.5e37f), 8.5e37f);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          low = fminf(low, x[j]);
-          high = fmaxf(high, x[j]);
-        }
-#pragma unroll
-        for (int d = kLanes / 2; d; d /= 2) {
-          low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
-          high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+          for (int j = 0; j < 4; ++j) {
+            x[j].x = x[j].x != x[j].x ? 0.f : fminf(fmaxf(x[j].x, -8.5e37f), 8.5e37f);
+            x[j].y = x[j].y != x[j].y ? 0.f : fminf(fmaxf(x[j].y, -8.5e37f), 8.5e37f);
+          }
+          range();
         }
         const Kv4Code code = kv4_code_of(low, high);
         const uint32_t word = kv4_encode8(x, code);
         if (real && !is_q) {
-          const int page = 1 << p.page_shift;
-          const int64_t at = slot >> p.page_shift;
-          const int row = static_cast<int>(slot & (page - 1));
-          const int head = h - q_heads - (is_v ? p.kv_heads : 0);
-          uint8_t* block = p.cache + ((at * kKv4Side + (is_v ? 1 : 0)) * p.kv_heads + head) * kv4_block_bytes(page, kDim);
-          *reinterpret_cast<uint32_t*>(block + static_cast<int64_t>(row) * (kDim / 2) + 4 * l) = word;
-          if (l == 0)
-            *reinterpret_cast<uint32_t*>(block + static_cast<int64_t>(page) * (kDim / 2) + 4 * row) =
-                pack2(code.scale, static_cast<float>(code.zero));
+          const int which = h - q_heads;                 // keys' heads, then values'
+          uint8_t* block = slot_page + which * block_bytes;
+          uint8_t* row = block + slot_row * (kDim / 2);
+          *reinterpret_cast<uint16_t*>(row + run0 / 2) = static_cast<uint16_t>(word);
+          *reinterpret_cast<uint16_t*>(row + run1 / 2) = static_cast<uint16_t>(word >> 16);
+          if (l == 0) *reinterpret_cast<uint32_t*>(block + page * (kDim / 2) + 4 * slot_row) = pack2(code.scale, code.zero);
         }
       }
     }
@@ -285,53 +323,60 @@ struct Kv4ReadParams {
   uint16_t* k;               // [tokens, kv_heads, dim]
   uint16_t* v;
   int64_t capacity;
-  int64_t rows;              // tokens * 2 * kv_heads
-  int kv_heads, page_shift;
+  int tokens, kv_heads, page_shift;
+  int chunks;                // pieces that the heads of one token are cut into, one warp each
 };
 
-// One lane group takes a head of a token: eight codes (one word) per lane become eight BF16 values, one
-// rounding each. Bound by memory (dim / 2 + 4 bytes read, 2 dim written per head).
+// One warp takes a piece of one token's heads (keys', then values'): eight codes (one word) per lane become eight BF16
+// values. Two codes behind a mask are the BF16 numbers 128 + code; the zero point comes off exactly and the product
+// with the scale is rounded once. Bound by memory (dim / 2 + 4 bytes read, 2 dim written per head).
 template <int kDim>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
-  constexpr int kLanes = kDim / 8, kBatch = 4;
+  constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 8;
   pdl_wait();
+  pdl_launch_dependents();
   const int page = 1 << p.page_shift;
-  const int l = threadIdx.x % kLanes;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (blockDim.x / kLanes);
-  const int64_t group = static_cast<int64_t>(blockIdx.x) * (blockDim.x / kLanes) + threadIdx.x / kLanes;
-  for (int64_t base = group; base < p.rows; base += groups * kBatch) {
+  const unsigned block_bytes = page * (kDim / 2 + 4);
+  const int warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int token = warp / p.chunks, chunk = warp % p.chunks;
+  if (token >= p.tokens) return;
+  const int lane = threadIdx.x % 32, l = lane % kLanes, sub = lane / kLanes;
+  const int heads = 2 * p.kv_heads, per_chunk = (heads + p.chunks - 1) / p.chunks;
+  const int first = chunk * per_chunk, end = min(heads, first + per_chunk);
+  const int64_t slot = p.slots[token];
+  if (slot >= p.capacity && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
+  const bool there = slot >= 0 && slot < p.capacity;
+  const uint8_t* src = p.cache + (there ? (slot >> p.page_shift) * heads * static_cast<int64_t>(block_bytes) : 0);
+  const int row = static_cast<int>(slot & (page - 1));
+  uint16_t* const k = p.k + static_cast<int64_t>(token) * p.kv_heads * kDim + 8 * l;
+  uint16_t* const v = p.v + static_cast<int64_t>(token) * p.kv_heads * kDim + 8 * l;
+  for (int base = first; base < end; base += kBatch * kHeadsPerStep) {
     uint32_t word[kBatch], pair[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int64_t row = base + i * groups;
-      word[i] = 0;
-      pair[i] = 0;                       // scale 0: the row reads as zeros
-      if (row < p.rows) {
-        const int64_t token = row / (2 * p.kv_heads);
-        const int which = static_cast<int>(row % (2 * p.kv_heads));
-        const int64_t slot = p.slots[token];
-        if (slot >= p.capacity && l == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
-        if (slot >= 0 && slot < p.capacity) {
-          const uint8_t* block = p.cache + ((slot >> p.page_shift) * kKv4Side * p.kv_heads + which) * kv4_block_bytes(page, kDim);
-          const int at = static_cast<int>(slot & (page - 1));
-          word[i] = *reinterpret_cast<const uint32_t*>(block + static_cast<int64_t>(at) * (kDim / 2) + 4 * l);
-          pair[i] = *reinterpret_cast<const uint32_t*>(block + static_cast<int64_t>(page) * (kDim / 2) + 4 * at);
-        }
+      const int h = base + i * kHeadsPerStep + sub;
+      word[i] = pair[i] = 0;                             // scale 0: the row reads as zeros
+      if (there && h < end) {
+        word[i] = *reinterpret_cast<const uint32_t*>(src + h * block_bytes + row * (kDim / 2) + 4 * l);
+        pair[i] = *reinterpret_cast<const uint32_t*>(src + h * block_bytes + page * (kDim / 2) + 4 * row);
       }
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int64_t row = base + i * groups;
-      if (row >= p.rows) break;
-      const int64_t token = row / (2 * p.kv_heads);
-      const int which = static_cast<int>(row % (2 * p.kv_heads));
-      const float scale = bf16_lo(pair[i]), zero = bf16_hi(pair[i]);
-      float x[8];
+      const int h = base + i * kHeadsPerStep + sub;
+      if (h >= end) continue;
+      const uint32_t scale = __byte_perm(pair[i], 0, 0x1010);
+      uint32_t zero = __byte_perm(pair[i], 0, 0x3232), x[4];
+      asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(zero) : "r"(0x43004300u));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = scale * (static_cast<float>((word[i] >> (4 * j)) & 15u) - zero);
-      uint16_t* dst = which < p.kv_heads ? p.k + (token * p.kv_heads + which) * kDim
-                                         : p.v + (token * p.kv_heads + which - p.kv_heads) * kDim;
-      *reinterpret_cast<uint4*>(dst + 8 * l) = pack8(x);
+      for (int j = 0; j < 4; ++j) {                      // components j and j + 4
+        x[j] = ((word[i] >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+        asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(x[j]) : "r"(zero));
+        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(x[j]) : "r"(scale));
+      }
+      uint16_t* dst = h < p.kv_heads ? k + h * kDim : v + (h - p.kv_heads) * kDim;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410),
+                                                  __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
     }
   }
 }
