@@ -849,18 +849,27 @@ int kv4_chunks(int tokens, long long steps, long long batch) {
   if (tokens >= sm_count() * 8 && chunks > batches) chunks = batches;
   return static_cast<int>(chunks < steps ? chunks : steps);
 }
+// Pieces of whole steps that `heads` heads are cut into when all heads of a token are to make about `chunks` pieces.
+int kv4_pieces(int heads, int per_step, long long all_steps, long long chunks) {
+  if (heads == 0) return 0;
+  const long long steps = (heads + per_step - 1) / per_step;
+  long long pieces = (steps * chunks + all_steps - 1) / all_steps;
+  const long long per_piece = ((steps + pieces - 1) / pieces) * per_step;
+  return static_cast<int>((heads + per_piece - 1) / per_piece);
+}
 template <int kDim, bool kNorm, bool kAppend>
 int launch_kv4_rows(Kv4RowParams p, ci8_stream_t stream) {
-  const int per_step = 32 / (kDim / 8);
-  const int heads = (p.q ? p.q_heads : 0) + p.kv_heads * (kAppend ? 2 : 1);
-  const long long steps = (heads + per_step - 1) / per_step;
+  const int per_step = 32 / (kDim / 8), sides = kAppend ? 2 : 1;
+  if (!p.q) p.q_heads = 0;
+  const long long steps = (p.q_heads + per_step - 1) / per_step + sides * ((p.kv_heads + per_step - 1) / per_step);
   const long long chunks = kv4_chunks(p.tokens, steps, 4);
-  const long long per_chunk = ((steps + chunks - 1) / chunks) * per_step;   // whole steps
-  p.chunks = static_cast<int>((heads + per_chunk - 1) / per_chunk);
-  const long long warps = static_cast<long long>(p.tokens) * p.chunks;
+  p.q_chunks = kv4_pieces(p.q_heads, per_step, steps, chunks);
+  p.kv_chunks = kv4_pieces(p.kv_heads, per_step, steps, chunks);
+  const long long warps = static_cast<long long>(p.tokens) * (p.q_chunks + sides * p.kv_chunks);
   const int per_cta = warps < 8 * sm_count() ? 1 : 8;
-  if (warps / per_cta >= 0x7fffffffll) return kInvalid;
-  return launch_pdl(kv4_rows_kernel<kDim, kNorm, kAppend>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
+  if (warps > 0x7fffff00ll) return kInvalid;
+  return launch_pdl(p.adjacent ? kv4_rows_kernel<kDim, kNorm, kAppend, true> : kv4_rows_kernel<kDim, kNorm, kAppend, false>,
+                    dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
 }
 template <int kDim>
 int launch_kv4_read(Kv4ReadParams p, ci8_stream_t stream) {
@@ -871,7 +880,7 @@ int launch_kv4_read(Kv4ReadParams p, ci8_stream_t stream) {
   p.chunks = static_cast<int>((heads + per_chunk - 1) / per_chunk);
   const long long warps = static_cast<long long>(p.tokens) * p.chunks;
   const int per_cta = warps < 8 * sm_count() ? 1 : 8;
-  if (warps / per_cta >= 0x7fffffffll) return kInvalid;
+  if (warps > 0x7fffff00ll) return kInvalid;
   return launch_pdl(kv4_read_kernel<kDim>, dim3(static_cast<unsigned>((warps + per_cta - 1) / per_cta)), 32 * per_cta, 0, stream, p);
 }
 template <bool kNorm, bool kAppend>

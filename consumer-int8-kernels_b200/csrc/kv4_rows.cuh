@@ -40,7 +40,8 @@ struct Kv4RowParams {
   int64_t capacity;          // pages * page_size
   int table_rows, rotary, axes, adjacent;
   int tokens, q_heads, kv_heads, page_shift;
-  int chunks;                // pieces that the heads of one token are cut into, one warp each
+  int q_chunks, kv_chunks;   // pieces that the heads of one token are cut into, one warp each: q_chunks of queries, then
+                             // kv_chunks of keys (and as many of values when appending)
   float eps, weight_offset;
 };
 
@@ -109,12 +110,6 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7]));
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w) { return make_float2(bf16_lo(w), bf16_hi(w)); }
-// x * cosine + partner * sine with every product and the sum rounded on its own. (The packed intrinsics are no barrier to
-// contraction; single products and sums with a rounding mode are.)
-__device__ __forceinline__ float2 turn2(float2 x, float2 cosine, float2 partner, float2 sine) {
-  return make_float2(__fadd_rn(__fmul_rn(x.x, cosine.x), __fmul_rn(partner.x, sine.x)),
-                     __fadd_rn(__fmul_rn(x.y, cosine.y), __fmul_rn(partner.y, sine.y)));
-}
 // Minimum and maximum that keep a NaN.
 __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
@@ -127,59 +122,57 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// One warp takes a piece of one token's heads (queries, keys and, when appending, values, in that order): the token's
-// angles and the norm's weights stay in registers, and up to kBatch heads per lane group are loaded before the first is
-// used. A lane holds two runs of four components. Turning components (i, i + rotary / 2), it holds both of a pair: runs
-// 4 l and rotary / 2 + 4 l, so the rotation needs no exchange between lanes; otherwise its runs are neighbours. FP32
-// throughout, two components to an instruction; products and sums of the rotation are rounded one by one (no FMA), so
-// that what is encoded does not depend on how a compiler contracts them. Bound by memory: 4 bytes per component of the
-// norm, 2 read and dim / 2 + 4 bytes per head written for what is appended.
-template <int kDim, bool kNorm, bool kAppend>
-__global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4RowParams p) {
+// One warp takes a piece of one token's query, key or value heads: the token's angles and the norm's weights stay in
+// registers, and up to kBatch heads per lane group are loaded before the first is used. A lane holds two runs of four
+// components. Turning components (i, i + rotary / 2), it holds both of a pair: runs 4 l and rotary / 2 + 4 l, so the
+// rotation needs no exchange between lanes; otherwise its runs are neighbours. FP32 throughout, two components to an
+// instruction where nothing speaks against it. Bound by memory: 4 bytes per component of the norm, 2 read and
+// dim / 2 + 4 bytes per head written for what is appended.
+template <int kDim, bool kNorm, bool kAppend, bool kAdjacent>
+__global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) {
   constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 4;
   pdl_wait();
   pdl_launch_dependents();
   const int warp = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  const int token = warp / p.chunks, chunk = warp % p.chunks;
+  const int chunks = p.q_chunks + p.kv_chunks * (kAppend ? 2 : 1);
+  const int token = warp / chunks;
+  int chunk = warp - token * chunks;
   if (token >= p.tokens) return;      // whole warps
+  const int kind = chunk < p.q_chunks ? 0 : chunk < p.q_chunks + p.kv_chunks ? 1 : 2;        // queries, keys, values
+  chunk -= kind == 0 ? 0 : kind == 1 ? p.q_chunks : p.q_chunks + p.kv_chunks;
   const int lane = threadIdx.x % 32, l = lane % kLanes, sub = lane / kLanes;
-  const int q_heads = p.q ? p.q_heads : 0;
-  const int heads = q_heads + p.kv_heads * (kAppend ? 2 : 1);
-  const int per_chunk = (heads + p.chunks - 1) / p.chunks;
+  const int heads = kind == 0 ? p.q_heads : p.kv_heads, pieces = kind == 0 ? p.q_chunks : p.kv_chunks;
+  const int per_chunk = (heads + pieces - 1) / pieces;
   const int first = chunk * per_chunk, end = min(heads, first + per_chunk);
-  const bool turns = l < p.rotary / 8;                  // rotary is 0 without a table
-  const int run0 = turns && !p.adjacent ? 4 * l : 8 * l, run1 = turns && !p.adjacent ? p.rotary / 2 + 4 * l : 8 * l + 4;
+  const bool turns = kind < 2 && l < p.rotary / 8;      // rotary is 0 without a table
+  const bool split = turns && !kAdjacent;
+  const int run0 = split ? 4 * l : 8 * l, run1 = split ? p.rotary / 2 + 4 * l : 8 * l + 4;
 
-  const uint16_t* const q_src = p.q ? p.q + token * p.q_stride : nullptr;
-  const uint16_t* const k_src = p.k + token * p.k_stride;
-  const uint16_t* const v_src = kAppend ? p.v + token * p.v_stride : nullptr;
+  const uint16_t* const src = (kind == 0 ? p.q + token * p.q_stride : kind == 1 ? p.k + token * p.k_stride : p.v + token * p.v_stride) + sub * kDim;
   uint2 raw[kBatch][2];
   auto load = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int h = base + i * kHeadsPerStep + sub;
+      const int h = base + i * kHeadsPerStep;
       raw[i][0] = raw[i][1] = make_uint2(0, 0);
-      if (h < end) {
-        const uint16_t* src = h < q_heads ? q_src + h * kDim
-                              : (!kAppend || h < q_heads + p.kv_heads) ? k_src + (h - q_heads) * kDim : v_src + (h - q_heads - p.kv_heads) * kDim;
-        raw[i][0] = *reinterpret_cast<const uint2*>(src + run0);
-        raw[i][1] = *reinterpret_cast<const uint2*>(src + run1);
+      if (h + sub < end) {
+        raw[i][0] = *reinterpret_cast<const uint2*>(src + h * kDim + run0);
+        raw[i][1] = *reinterpret_cast<const uint2*>(src + h * kDim + run1);
       }
     }
   };
   load(first);
 
-  // The token's angles: y[i] = x[i] * cosine[i] + partner[i] * sine[i] over pairs of components.
-  float2 cosine[4], sine[4];
+  // The token's angles: this lane's four pairs.
+  float c[4] = {}, s[4] = {};
   bool bad = false;
   if (p.cos_sin) {
     for (int a = 0; a < p.axes; ++a) {
       const int64_t place = p.positions[static_cast<int64_t>(a) * p.tokens + token];
       bad |= place < 0 || place >= p.table_rows;
     }
-    float c[4] = {}, s[4] = {};
-    const int f = 4 * l, pairs = p.rotary / 2;           // this lane's four pairs, either way of pairing
-    if (turns && !bad) {
+    const int f = 4 * l, pairs = p.rotary / 2;
+    if (l < p.rotary / 8 && !bad) {
       if (!p.axis_of) {
         const float* row = p.cos_sin + p.positions[token] * p.rotary + f;
         const float4 cs = *reinterpret_cast<const float4*>(row), sn = *reinterpret_cast<const float4*>(row + pairs);
@@ -199,55 +192,44 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4RowParams p) {
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int e = j % 2 * 2;                           // not adjacent: components 0..3 with 4..7
-      cosine[j] = p.adjacent ? make_float2(c[j], c[j]) : make_float2(c[e], c[e + 1]);
-      sine[j] = p.adjacent ? make_float2(-s[j], s[j]) : j < 2 ? make_float2(-s[e], -s[e + 1]) : make_float2(s[e], s[e + 1]);
-    }
   }
   bad = __any_sync(0xffffffffu, bad);
   if (bad && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
 
-  float2 q_weight[4], k_weight[4];
-  if constexpr (kNorm) {
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const uint16_t* weight = side ? p.k_weight : p.q_weight;
-      float2(&to)[4] = side ? k_weight : q_weight;
-      if (weight) {
-        const uint2 a = *reinterpret_cast<const uint2*>(weight + run0), b = *reinterpret_cast<const uint2*>(weight + run1);
-        const float2 offset = make_float2(p.weight_offset, p.weight_offset);
-        to[0] = __fadd2_rn(unpack2(a.x), offset);
-        to[1] = __fadd2_rn(unpack2(a.y), offset);
-        to[2] = __fadd2_rn(unpack2(b.x), offset);
-        to[3] = __fadd2_rn(unpack2(b.y), offset);
-      }
-    }
+  float2 weight[4];
+  const uint16_t* const weights = kNorm ? (kind == 0 ? p.q_weight : p.k_weight) : nullptr;
+  if (weights) {
+    const uint2 a = *reinterpret_cast<const uint2*>(weights + run0), b = *reinterpret_cast<const uint2*>(weights + run1);
+    const float2 offset = make_float2(p.weight_offset, p.weight_offset);
+    weight[0] = __fadd2_rn(unpack2(a.x), offset);
+    weight[1] = __fadd2_rn(unpack2(a.y), offset);
+    weight[2] = __fadd2_rn(unpack2(b.x), offset);
+    weight[3] = __fadd2_rn(unpack2(b.y), offset);
   }
 
-  uint8_t* slot_page = nullptr;                          // the slot's page, null: not stored
+  // Where the heads go: the outputs' rows, or the slot's page (null: not stored).
+  uint16_t* const dst = kind == 0 ? p.q_out + token * p.q_out_stride + sub * kDim : kAppend ? nullptr : p.k_out + token * p.k_out_stride + sub * kDim;
+  uint8_t* slot_page = nullptr;
   int slot_row = 0;
   const int page = 1 << p.page_shift;
   const unsigned block_bytes = page * (kDim / 2 + 4);    // at most 32 KB
-  if constexpr (kAppend) {
+  if (kAppend && kind > 0) {
     const int64_t slot = p.slots[token];
     if (slot >= p.capacity && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
-    if (slot >= 0 && slot < p.capacity && !bad) {
-      slot_page = p.cache + (slot >> p.page_shift) * kKv4Side * p.kv_heads * static_cast<int64_t>(block_bytes);
-      slot_row = static_cast<int>(slot & (page - 1));
-    }
+    if (slot < 0 || slot >= p.capacity || bad) return;
+    slot_page = p.cache + ((slot >> p.page_shift) * kKv4Side + kind - 1) * p.kv_heads * static_cast<int64_t>(block_bytes);
+    slot_row = static_cast<int>(slot & (page - 1));
   }
 
   for (int base = first; base < end; base += kBatch * kHeadsPerStep) {
     if (base > first) load(base);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (base + i * kHeadsPerStep >= end) break;        // the same for the whole warp
-      const int h = base + i * kHeadsPerStep + sub;
-      const bool is_q = h < q_heads, is_v = kAppend && h >= q_heads + p.kv_heads, real = h < end;
+      const int h = base + i * kHeadsPerStep;
+      if (h >= end) break;                               // the same for the whole warp
+      const bool real = h + sub < end;
       float2 x[4] = {unpack2(raw[i][0].x), unpack2(raw[i][0].y), unpack2(raw[i][1].x), unpack2(raw[i][1].y)};
-      if constexpr (kNorm) {
+      if (weights) {
         float2 squares = __fmul2_rn(x[0], x[0]);
 #pragma unroll
         for (int j = 1; j < 4; ++j) squares = __ffma2_rn(x[j], x[j], squares);
@@ -255,63 +237,71 @@ __global__ void __launch_bounds__(256) kv4_rows_kernel(const Kv4RowParams p) {
 #pragma unroll
         for (int d = kLanes / 2; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         const float unit = rsqrtf(sum * (1.f / kDim) + p.eps);
-        if (is_q ? p.q_weight : p.k_weight) {
-          const float2 unit2 = make_float2(unit, unit);
+        const float2 unit2 = make_float2(unit, unit);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = __fmul2_rn(__fmul2_rn(x[j], unit2), is_q ? q_weight[j] : k_weight[j]);
+        for (int j = 0; j < 4; ++j) x[j] = __fmul2_rn(__fmul2_rn(x[j], unit2), weight[j]);
+      }
+      if (turns) {
+        // Products and sums rounded one by one (single ones with a rounding mode; the packed ones may be contracted), so
+        // that what is encoded does not depend on how a compiler contracts them.
+        if constexpr (kAdjacent) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            x[j] = make_float2(__fsub_rn(__fmul_rn(x[j].x, c[j]), __fmul_rn(x[j].y, s[j])),
+                               __fadd_rn(__fmul_rn(x[j].y, c[j]), __fmul_rn(x[j].x, s[j])));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 a = x[j], b = x[j + 2];
+            x[j] = make_float2(__fsub_rn(__fmul_rn(a.x, c[2 * j]), __fmul_rn(b.x, s[2 * j])),
+                               __fsub_rn(__fmul_rn(a.y, c[2 * j + 1]), __fmul_rn(b.y, s[2 * j + 1])));
+            x[j + 2] = make_float2(__fadd_rn(__fmul_rn(b.x, c[2 * j]), __fmul_rn(a.x, s[2 * j])),
+                                   __fadd_rn(__fmul_rn(b.y, c[2 * j + 1]), __fmul_rn(a.y, s[2 * j + 1])));
+          }
         }
       }
-      if (turns && !is_v) {
-        float2 partner[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) partner[j] = p.adjacent ? make_float2(x[j].y, x[j].x) : x[j ^ 2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = turn2(x[j], cosine[j], partner[j], sine[j]);
+      if (!kAppend || kind == 0) {
+        if (real) {
+          uint2 a = make_uint2(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y)), b = make_uint2(pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y));
+          if (bad) a = b = make_uint2(0x7fff7fffu, 0x7fff7fffu);   // a position outside the table: NaN
+          *reinterpret_cast<uint2*>(dst + h * kDim + run0) = a;
+          *reinterpret_cast<uint2*>(dst + h * kDim + run1) = b;
+        }
+        continue;
       }
-      if ((!kAppend || is_q) && real) {
-        uint2 a = make_uint2(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y)), b = make_uint2(pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y));
-        if (bad) a = b = make_uint2(0x7fff7fffu, 0x7fff7fffu);   // a position outside the table: NaN
-        uint16_t* dst = is_q ? p.q_out + token * p.q_out_stride + h * kDim : p.k_out + token * p.k_out_stride + (h - q_heads) * kDim;
-        *reinterpret_cast<uint2*>(dst + run0) = a;
-        *reinterpret_cast<uint2*>(dst + run1) = b;
-      }
-      if constexpr (kAppend) {
-        if (!slot_page || base + (i + 1) * kHeadsPerStep <= q_heads) continue;   // whole warps: nothing to encode here
-        float low = 0.f, high = 0.f;
-        auto range = [&]() {
-          low = high = 0.f;
+      float low, high;
+      auto range = [&]() {
+        low = high = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            low = min_nan(low, min_nan(x[j].x, x[j].y));
-            high = max_nan(high, max_nan(x[j].x, x[j].y));
-          }
+        for (int j = 0; j < 4; ++j) {
+          low = min_nan(low, min_nan(x[j].x, x[j].y));
+          high = max_nan(high, max_nan(x[j].x, x[j].y));
+        }
 #pragma unroll
-          for (int d = kLanes / 2; d; d /= 2) {
-            low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
-            high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
-          }
-        };
+        for (int d = kLanes / 2; d; d /= 2) {
+          low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, d));
+          high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, d));
+        }
+      };
+      range();
+      if (__any_sync(0xffffffffu, !(low >= -8.5e37f && high <= 8.5e37f))) {
+        // NaN counts as 0 and infinities as the largest value whose range still fits FP32, so that one such
+        // component cannot spoil the scale and with it the whole head
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j].x = x[j].x != x[j].x ? 0.f : fminf(fmaxf(x[j].x, -8.5e37f), 8.5e37f);
+          x[j].y = x[j].y != x[j].y ? 0.f : fminf(fmaxf(x[j].y, -8.5e37f), 8.5e37f);
+        }
         range();
-        if (__any_sync(0xffffffffu, !(low >= -8.5e37f && high <= 8.5e37f))) {
-          // NaN counts as 0 and infinities as the largest value whose range still fits FP32, so that one such
-          // component cannot spoil the scale and with it the whole head
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j].x = x[j].x != x[j].x ? 0.f : fminf(fmaxf(x[j].x, -8.5e37f), 8.5e37f);
-            x[j].y = x[j].y != x[j].y ? 0.f : fminf(fmaxf(x[j].y, -8.5e37f), 8.5e37f);
-          }
-          range();
-        }
-        const Kv4Code code = kv4_code_of(low, high);
-        const uint32_t word = kv4_encode8(x, code);
-        if (real && !is_q) {
-          const int which = h - q_heads;                 // keys' heads, then values'
-          uint8_t* block = slot_page + which * block_bytes;
-          uint8_t* row = block + slot_row * (kDim / 2);
-          *reinterpret_cast<uint16_t*>(row + run0 / 2) = static_cast<uint16_t>(word);
-          *reinterpret_cast<uint16_t*>(row + run1 / 2) = static_cast<uint16_t>(word >> 16);
-          if (l == 0) *reinterpret_cast<uint32_t*>(block + page * (kDim / 2) + 4 * slot_row) = pack2(code.scale, code.zero);
-        }
+      }
+      const Kv4Code code = kv4_code_of(low, high);
+      const uint32_t word = kv4_encode8(x, code);
+      if (real) {
+        uint8_t* block = slot_page + (h + sub) * block_bytes;
+        uint8_t* row = block + slot_row * (kDim / 2);
+        *reinterpret_cast<uint16_t*>(row + run0 / 2) = static_cast<uint16_t>(word);
+        *reinterpret_cast<uint16_t*>(row + run1 / 2) = static_cast<uint16_t>(word >> 16);
+        if (l == 0) *reinterpret_cast<uint32_t*>(block + page * (kDim / 2) + 4 * slot_row) = pack2(code.scale, code.zero);
       }
     }
   }
