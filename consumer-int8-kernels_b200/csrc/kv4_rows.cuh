@@ -123,7 +123,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // One warp takes a piece of one token's query, key or value heads: the token's angles and the norm's weights stay in
-// registers, and up to kBatch heads per lane group are loaded before the first is used. A lane holds two runs of four
+// registers, and kBatch heads per lane group are loaded ahead of the one in work. A lane holds two runs of four
 // components. Turning components (i, i + rotary / 2), it holds both of a pair: runs 4 l and rotary / 2 + 4 l, so the
 // rotation needs no exchange between lanes; otherwise its runs are neighbours. FP32 throughout, two components to an
 // instruction where nothing speaks against it. Bound by memory: 4 bytes per component of the norm, 2 read and
@@ -150,18 +150,21 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) 
 
   const uint16_t* const src = (kind == 0 ? p.q + token * p.q_stride : kind == 1 ? p.k + token * p.k_stride : p.v + token * p.v_stride) + sub * kDim;
   uint2 raw[kBatch][2];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int h = base + i * kHeadsPerStep;
-      raw[i][0] = raw[i][1] = make_uint2(0, 0);
-      if (h + sub < end) {
+  auto load = [&](int i, int h) {
+    raw[i][0] = raw[i][1] = make_uint2(0, 0);
+    if (h + sub < end) {
+      if constexpr (kAdjacent) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src + h * kDim + run0);
+        raw[i][0] = make_uint2(w.x, w.y);
+        raw[i][1] = make_uint2(w.z, w.w);
+      } else {
         raw[i][0] = *reinterpret_cast<const uint2*>(src + h * kDim + run0);
         raw[i][1] = *reinterpret_cast<const uint2*>(src + h * kDim + run1);
       }
     }
   };
-  load(first);
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) load(i, first + i * kHeadsPerStep);
 
   // The token's angles: this lane's four pairs.
   float c[4] = {}, s[4] = {};
@@ -222,13 +225,13 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) 
   }
 
   for (int base = first; base < end; base += kBatch * kHeadsPerStep) {
-    if (base > first) load(base);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int h = base + i * kHeadsPerStep;
       if (h >= end) break;                               // the same for the whole warp
       const bool real = h + sub < end;
       float2 x[4] = {unpack2(raw[i][0].x), unpack2(raw[i][0].y), unpack2(raw[i][1].x), unpack2(raw[i][1].y)};
+      load(i, h + kBatch * kHeadsPerStep);
       if (weights) {
         float2 squares = __fmul2_rn(x[0], x[0]);
 #pragma unroll
@@ -264,8 +267,12 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) 
         if (real) {
           uint2 a = make_uint2(pack2(x[0].x, x[0].y), pack2(x[1].x, x[1].y)), b = make_uint2(pack2(x[2].x, x[2].y), pack2(x[3].x, x[3].y));
           if (bad) a = b = make_uint2(0x7fff7fffu, 0x7fff7fffu);   // a position outside the table: NaN
-          *reinterpret_cast<uint2*>(dst + h * kDim + run0) = a;
-          *reinterpret_cast<uint2*>(dst + h * kDim + run1) = b;
+          if constexpr (kAdjacent) {
+            *reinterpret_cast<uint4*>(dst + h * kDim + run0) = make_uint4(a.x, a.y, b.x, b.y);
+          } else {
+            *reinterpret_cast<uint2*>(dst + h * kDim + run0) = a;
+            *reinterpret_cast<uint2*>(dst + h * kDim + run1) = b;
+          }
         }
         continue;
       }
