@@ -26,16 +26,20 @@
 
 namespace ci8 {
 
-constexpr int kKv4Tile = 32;                                    // tokens per ring stage
 constexpr int kKv4CounterBytes = 4096;                          // arrival counters at the head of the workspace
 constexpr int kKv4MaxCtas = kKv4CounterBytes / 4;
 
 template <int kDim, int kQ>                                     // kQ: groups of eight query rows per warp
 struct Kv4SingleConfig {
   static constexpr int kRows = 8 * kQ;
-  static constexpr int kWarps = kDim * kQ <= 128 ? 16 : 8;      // registers: output and queries take kDim * kQ * 3 / 8 each thread
-  static constexpr int kCodeBytes = kKv4Tile * kDim / 2;
-  static constexpr int kPairBytes = kKv4Tile * 4;
+  // Tokens per ring stage: 64 halve what a tile costs beside its products, 32 are what the ring has room for at dim 256.
+  // Warps: as many as the registers allow (output and queries take kDim * kQ * 3 / 8 a thread). Measured (us, 64 sequences of
+  // up to 8192 keys, 4 heads a key head): 32 tokens and 16 warps 91, 64 and 12 83, 64 and 8 87, 32 and 12 94.
+  static constexpr int kTile = kDim <= 128 ? 64 : 32;
+  static constexpr int kWarps = kDim * kQ == 64 ? 16 : kDim * kQ == 128 || kDim == 256 && kQ == 1 ? 12 : 8;
+  static constexpr int kParts = kTile / 16;                     // a part lies on one page
+  static constexpr int kCodeBytes = kTile * kDim / 2;
+  static constexpr int kPairBytes = kTile * 4;
   static constexpr int kStageBytes = 2 * (kCodeBytes + kPairBytes);
   static constexpr int kRing = 204 * 1024 / (kWarps * kStageBytes);
   static constexpr int kStages = kRing > 6 ? 6 : kRing;
@@ -127,21 +131,33 @@ template <int kDst, int kSrc>
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(kDst), "n"(kSrc) : "memory");
 }
-// Code rows of half a tile, 512 bytes at a time: kCopies copies at kDst + 512 * i.
+// Code rows, 512 bytes at a time: kCopies copies at kDst + 512 * i, every other one from dst_odd.
 template <int kCopies, int kDst, int i = 0>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src) {
+__device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t dst_odd, const uint8_t* src) {
   if constexpr (i < kCopies) {
-    copy16<kDst + 512 * i, 512 * i>(dst, src);
-    copy_rows<kCopies, kDst, i + 1>(dst, src);
+    copy16<kDst + 512 * i, 512 * i>(i % 2 ? dst_odd : dst, src);
+    copy_rows<kCopies, kDst, i + 1>(dst, dst_odd, src);
   }
 }
 // Of those rows the first `rows`; the lane's row of the first copy is lane_row, and a copy covers kPerCopy.
 template <int kCopies, int kDst, int kPerCopy, int i = 0>
-__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t* src, int rows, int lane_row) {
+__device__ __forceinline__ void copy_rows(uint32_t dst, uint32_t dst_odd, const uint8_t* src, int rows, int lane_row) {
   if constexpr (i < kCopies) {
-    copy16<kDst + 512 * i, 512 * i>(dst, src, lane_row + i * kPerCopy < rows ? 16 : 0);
-    copy_rows<kCopies, kDst, kPerCopy, i + 1>(dst, src, rows, lane_row);
+    copy16<kDst + 512 * i, 512 * i>(i % 2 ? dst_odd : dst, src, lane_row + i * kPerCopy < rows ? 16 : 0);
+    copy_rows<kCopies, kDst, kPerCopy, i + 1>(dst, dst_odd, src, rows, lane_row);
   }
+}
+// The places in shared memory that the lanes (g, c) of a warp read together: 16 bytes (dim 64: 8) of the keys of rows
+// kv4_row(g) at c, 16 (8, 4) bytes of the values of the rows kv4_row(2c) or kv4_row(2c + 1) at g. Which token a row of
+// S^T stands for is free, and so is the order of a row's 16-byte pieces (piece ^ kv4_turn(row)): chosen such that the
+// eight (sixteen, thirty-two) lanes of one access lie in different banks for keys and for values.
+template <int kDim>
+__device__ __forceinline__ int kv4_row(int g) {
+  return kDim == 64 ? g ^ (g >> 2 & 1) : kDim == 128 ? g ^ (g >> 1 & 1) : g >> 1 | (g & 1) << 2;
+}
+template <int kDim>
+__device__ __forceinline__ int kv4_turn(int row) {
+  return kDim == 64 ? 0 : kDim == 128 ? row >> 1 & 2 : ((row & 3) << 1) ^ (row & 4);
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -155,14 +171,16 @@ __device__ __forceinline__ int kv4_block_keys(const Kv4Sequence& s, const Kv4Div
   const int last = min(s.rows * static_cast<int>(group.d), (block + 1) * rows_per_block) - 1;
   return max(0, s.keys - s.rows + group.quotient(last) + 1);
 }
-__device__ __forceinline__ int kv4_block_tiles(int keys) { return max(1, (keys + kKv4Tile - 1) / kKv4Tile); }
+template <int kTile>
+__device__ __forceinline__ int kv4_block_tiles(int keys) { return max(1, (keys + kTile - 1) / kTile); }
 // Tiles of one key head of a sequence.
+template <int kTile>
 __device__ __forceinline__ long long kv4_head_tiles(const Kv4Sequence& s, const Kv4Divisor& group, int rows_per_block, int most_rows) {
   const int rows = s.rows * static_cast<int>(group.d);
   if (rows == 0 || rows > most_rows) return 0;
   long long tiles = 0;
 #pragma unroll 1
-  for (int block = 0; block * rows_per_block < rows; ++block) tiles += kv4_block_tiles(kv4_block_keys(s, group, rows_per_block, block));
+  for (int block = 0; block * rows_per_block < rows; ++block) tiles += kv4_block_tiles<kTile>(kv4_block_keys(s, group, rows_per_block, block));
   return tiles;
 }
 
@@ -178,6 +196,7 @@ template <int kDim, int kQ>
 __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4_single_kernel(const Kv4SingleParams params) {
   using Cfg = Kv4SingleConfig<kDim, kQ>;
   constexpr int kWarps = Cfg::kWarps, kThreads = kWarps * 32, kStages = Cfg::kStages, kRows = Cfg::kRows;
+  constexpr int kTile = Cfg::kTile, kParts = Cfg::kParts;
   constexpr int kKWords = kDim / 32;                     // a lane's words of a key row
   constexpr int kVWords = kDim / 64;                     // a lane's words of a value row
   constexpr int kLoad = kKWords > 4 ? 4 : kKWords;
@@ -202,7 +221,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   const int share = (p.batch + kThreads - 1) / kThreads;
   long long scan = 0;
   for (int b = thread * share; b < min(p.batch, (thread + 1) * share); ++b)
-    scan += kv4_head_tiles(kv4_sequence(p, b), p.group, kRows, params.most_rows) * p.kv_heads;
+    scan += kv4_head_tiles<kTile>(kv4_sequence(p, b), p.group, kRows, params.most_rows) * p.kv_heads;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const long long other = __shfl_up_sync(0xffffffffu, scan, d);
@@ -247,7 +266,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     unsigned per_head = 0;
     for (b = (w * 32 + t) * share;; ++b) {
       seq = kv4_sequence(p, b);
-      per_head = static_cast<unsigned>(kv4_head_tiles(seq, p.group, kRows, params.most_rows));
+      per_head = static_cast<unsigned>(kv4_head_tiles<kTile>(seq, p.group, kRows, params.most_rows));
       if (rest < per_head * p.kv_heads) break;
       rest -= per_head * p.kv_heads;
     }
@@ -255,30 +274,37 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     rest -= head * per_head;
     for (block = 0;; ++block) {
       keys = kv4_block_keys(seq, p.group, kRows, block);
-      tiles = kv4_block_tiles(keys);
+      tiles = kv4_block_tiles<kTile>(keys);
       if (rest < static_cast<unsigned>(tiles)) break;
       rest -= tiles;
     }
     tile = rest;
   }
 
-  // ---- the loader's side of the ring: the tiles of the range in order, copied by the lanes in pieces of 16 bytes (a tile
-  // touches one page, or two of 16 tokens); the lanes hold the next 32 page numbers of the sequence
+  // ---- the loader's side of the ring: the tiles of the range in order, copied by the lanes in pieces of 16 bytes; the
+  // lanes hold the next 32 page numbers of the sequence
   const int page = 1 << p.page_shift;
   const unsigned block_bytes = page * (kDim / 2 + 4), page_bytes = block_bytes * kKv4Side * p.kv_heads;   // at most 70 MB
   const uint32_t ring_base = smem_u32(ring) + warp * kStages * Cfg::kStageBytes;
-  const bool two_parts = page < kKv4Tile;
+  const bool small_page = page < kTile;                  // a tile touches several pages
   constexpr int kRowPieces = kDim / 32;                  // 16-byte pieces of a code row
-  const int lane_row = lane / kRowPieces;                // the lane's row among those one copy instruction covers
-  const uint32_t lane_code = ring_base + 16 * lane;
-  const unsigned value_lane = p.kv_heads * block_bytes + 16 * lane;
-  const int pair_token = 4 * (lane & 7);
-  const unsigned pair_offset = page * (kDim / 2) + 4 * pair_token + (lane & 8 ? p.kv_heads * block_bytes : 0);
-  const uint32_t pair_dst = ring_base + Cfg::kCodeBytes + 4 * pair_token + (lane & 8 ? Cfg::kCodeBytes + Cfg::kPairBytes : 0);
+  constexpr int kCopies = kRowPieces / 2, kPerCopy = 32 / kRowPieces;          // copies for a part's codes, rows a copy covers
+  constexpr int kValues = Cfg::kCodeBytes + Cfg::kPairBytes;
+  const int lane_row = lane / kRowPieces;                // the lane's row among those one copy covers
+  // Pieces are stored in an order that depends on the row, so that the lanes that read together read different banks
+  // (kv4_turn); at dim 256 every other copy has its rows' bit 2 set, which moves its pieces by 4.
+  const int lane_piece = lane % kRowPieces ^ kv4_turn<kDim>(lane_row);
+  const uint32_t lane_code = ring_base + 16 * (lane_row * kRowPieces + lane_piece);
+  const uint32_t lane_code_odd = ring_base + 16 * (lane_row * kRowPieces + (kDim == 256 ? lane_piece ^ 4 : lane_piece));
+  const unsigned value_offset = p.kv_heads * block_bytes;
+  // the pairs: a lane takes four tokens' of one side
+  const int pair_token = 4 * (lane % (kTile / 4)), pair_side = lane / (kTile / 4);
+  const unsigned pair_offset = page * (kDim / 2) + (pair_side ? value_offset : 0);
+  const uint32_t pair_dst = ring_base + Cfg::kCodeBytes + 4 * pair_token + pair_side * kValues;
   const uint8_t* head_src = nullptr;
   int window = -1, window_first = 0;
   auto load_window = [&]() {
-    window_first = tile * kKv4Tile >> p.page_shift;      // even when a tile touches two pages
+    window_first = tile * kTile >> p.page_shift;
     const int index = window_first + lane;
     window = static_cast<int64_t>(index) << p.page_shift < keys ? p.block_table[static_cast<int64_t>(b) * p.width + index] : -1;
   };
@@ -286,45 +312,50 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     head_src = p.cache + static_cast<uint64_t>(head) * block_bytes;
     load_window();
   };
+  auto page_src = [&](int id) { return head_src + static_cast<uint64_t>(static_cast<unsigned>(id)) * page_bytes; };
   auto issue = [&](int stage) {
-    const int token = tile * kKv4Tile;
-    const int rows = min(kKv4Tile, keys - token);        // none or fewer: rows that see nothing
-    int index = (token >> p.page_shift) - window_first;
-    if (index >= 32) {
-      load_window();
-      index = 0;
-    }
-    const int page0 = __shfl_sync(0xffffffffu, window, index), page1 = __shfl_sync(0xffffffffu, window, index + (two_parts ? 1 : 0));
-    bool good0 = static_cast<unsigned>(page0) < static_cast<unsigned>(p.pages);
-    bool good1 = static_cast<unsigned>(page1) < static_cast<unsigned>(p.pages);
-    if (((rows > 0 && !good0) || (rows > 16 && !good1)) && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
-    good0 = good0 && rows > 0;
-    good1 = good1 && rows > 16;
-    if (lane == 0) infos[warp][stage] = make_int4(b, head, block, (tile << 3) | (good0 ? 1 : 0) | (good1 ? 2 : 0) | (tile == tiles - 1 ? 4 : 0));
-    const int row = token & (page - 1);
-    const uint8_t* src0 = head_src + static_cast<uint64_t>(static_cast<unsigned>(good0 ? page0 : 0)) * page_bytes + row * (kDim / 2);
-    const uint8_t* src1 = two_parts ? head_src + static_cast<uint64_t>(static_cast<unsigned>(good1 ? page1 : 0)) * page_bytes : src0 + 16 * (kDim / 2);
-    constexpr int kCopies = kRowPieces / 2, kPerCopy = 32 / kRowPieces;        // copies for 16 rows of codes, rows a copy covers
-    constexpr int kValues = Cfg::kCodeBytes + Cfg::kPairBytes;
-    const uint32_t dst = lane_code + stage * Cfg::kStageBytes;
-    // the pairs: lanes 0..7 the keys', 8..15 the values', four tokens each
-    const uint8_t* pair_src = (two_parts && pair_token >= 16 ? src1 - 64 : src0 + row * (4 - kDim / 2)) + pair_offset;
-    const uint32_t pair_at = pair_dst + stage * Cfg::kStageBytes;
-    if (rows >= kKv4Tile && good0 && good1) {
-      copy_rows<kCopies, 0>(dst, src0 + 16 * lane);
-      copy_rows<kCopies, 512 * kCopies>(dst, src1 + 16 * lane);
-      copy_rows<kCopies, kValues>(dst, src0 + value_lane);
-      copy_rows<kCopies, kValues + 512 * kCopies>(dst, src1 + value_lane);
-      if (lane < 16) copy16<0, 0>(pair_at, pair_src);
+    const int token = tile * kTile;
+    const int rows = min(kTile, keys - token);           // none or fewer: rows that see nothing
+    if (((token + kTile - 1) >> p.page_shift) - window_first >= 32) load_window();
+    const int pair_at = token + pair_token;
+    int id = __shfl_sync(0xffffffffu, window, (pair_at >> p.page_shift) - window_first);
+    const bool wanted = token + (pair_token & ~15) < keys, good = wanted && static_cast<unsigned>(id) < static_cast<unsigned>(p.pages);
+    const uint32_t goods = __ballot_sync(0xffffffffu, good);
+    if (__any_sync(0xffffffffu, wanted && !good) && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
+    if (!good) id = 0;
+    const uint8_t* const pair_src = page_src(id) + pair_offset + 4 * (pair_at & (page - 1));
+    const uint32_t dst = lane_code + stage * Cfg::kStageBytes, dst_odd = lane_code_odd + stage * Cfg::kStageBytes;
+    const uint32_t to_pair = pair_dst + stage * Cfg::kStageBytes;
+    int parts = 0;                                       // of this tile that are there
+#pragma unroll
+    for (int r = 0; r < kParts; ++r) parts |= (goods >> (4 * r) & 1) << r;
+    if (lane == 0) infos[warp][stage] = make_int4(b, head, block, (tile << (kParts + 1)) | (tile == tiles - 1 ? 1 << kParts : 0) | parts);
+    const uint8_t* src = page_src(__shfl_sync(0xffffffffu, id, 0)) + (token & (page - 1)) * (kDim / 2) + 16 * lane;
+    if (rows == kTile && goods == ~0u) {
+      if (pair_side < 2) copy16<0, 0>(to_pair, pair_src);
+      if (!small_page) {
+        copy_rows<kCopies * kParts, 0>(dst, dst_odd, src);
+        copy_rows<kCopies * kParts, kValues>(dst, dst_odd, src + value_offset);
+      } else {
+#pragma unroll
+        for (int r = 0; r < kParts; ++r) {
+          const int at = token + 16 * r;
+          src = page_src(__shfl_sync(0xffffffffu, window, (at >> p.page_shift) - window_first)) + (at & (page - 1)) * (kDim / 2) + 16 * lane;
+          copy_rows<kCopies, 0>(dst + 8 * kDim * r, dst_odd + 8 * kDim * r, src);
+          copy_rows<kCopies, kValues>(dst + 8 * kDim * r, dst_odd + 8 * kDim * r, src + value_offset);
+        }
+      }
     } else {
       // rows behind the last key or on a page that cannot be followed are filled with zeros: scale 0, zero point 0
       // (their source is an address that is not read: a copy of no bytes)
-      const int rows0 = good0 ? rows : 0, rows1 = good1 ? rows - 16 : 0;
-      copy_rows<kCopies, 0, kPerCopy>(dst, src0 + 16 * lane, rows0, lane_row);
-      copy_rows<kCopies, 512 * kCopies, kPerCopy>(dst, src1 + 16 * lane, rows1, lane_row);
-      copy_rows<kCopies, kValues, kPerCopy>(dst, src0 + value_lane, rows0, lane_row);
-      copy_rows<kCopies, kValues + 512 * kCopies, kPerCopy>(dst, src1 + value_lane, rows1, lane_row);
-      if (lane < 16) copy16<0, 0>(pair_at, pair_src, 4 * max(0, min(4, pair_token >= 16 ? rows1 + 16 - pair_token : rows0 - pair_token)));
+#pragma unroll 1
+      for (int r = 0; r < kParts; ++r) {
+        const int at = token + 16 * r, part_rows = parts >> r & 1 ? rows - 16 * r : 0;
+        src = page_src(__shfl_sync(0xffffffffu, id, 4 * r)) + (at & (page - 1)) * (kDim / 2) + 16 * lane;
+        copy_rows<kCopies, 0, kPerCopy>(dst + 8 * kDim * r, dst_odd + 8 * kDim * r, src, part_rows, lane_row);
+        copy_rows<kCopies, kValues, kPerCopy>(dst + 8 * kDim * r, dst_odd + 8 * kDim * r, src + value_offset, part_rows, lane_row);
+      }
+      if (pair_side < 2) copy16<0, 0>(to_pair, pair_src, good ? 4 * max(0, min(4, rows - pair_token)) : 0);
     }
     if (++tile == tiles) {                               // the next block of rows, head or sequence
       tile = 0;
@@ -339,7 +370,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       }
       if (b < p.batch) {
         keys = kv4_block_keys(seq, p.group, kRows, block);
-        tiles = kv4_block_tiles(keys);
+        tiles = kv4_block_tiles<kTile>(keys);
         begin_unit();
       }
     }
@@ -356,10 +387,15 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   int cur_b = 0, cur_head = 0, cur_block = 0, cur_tile = 0, cur_rows = 0, cur_start = 0, cur_keys = 0, first_tile = 0;
   int least = 0;
   bool fresh = true;
-  const int turned = g ^ ((g >> 1) & 1);                 // which token of eight a row of S^T holds: spreads the reads over the banks
+  const int turned = kv4_row<kDim>(g);                   // which token of eight a row of S^T holds
+  const int t_even = kv4_row<kDim>(2 * c), t_odd = kv4_row<kDim>(2 * c + 1);
+  const int key_at = turned * (kDim / 2) + (kDim == 64 ? 8 * c : 16 * (c ^ kv4_turn<kDim>(turned)));
+  auto value_at = [&](int row) {
+    return row * (kDim / 2) + (kDim == 64 ? 4 * g : kDim == 128 ? 16 * (g >> 1 ^ kv4_turn<kDim>(row)) + 8 * (g & 1) : 16 * (g ^ kv4_turn<kDim>(row)));
+  };
+  const int even_at = value_at(t_even), odd_at = value_at(t_odd);
   uint32_t ones;                                         // kept in a register: an immediate would cost a second instruction
   asm volatile("mov.b32 %0, 0x64006400;" : "=r"(ones));
-  const int t_even = (2 * c) ^ (c & 1), t_odd = (2 * c + 1) ^ (c & 1);
 
   // Leaves this warp's maximum, sum (in piece_m, piece_l) and output of every row.
   auto write_piece = [&](int piece, float* dst) {
@@ -474,7 +510,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     int4 info = make_int4(0, 0, 0, 0);
     if (it >= 0) {
       info = infos[warp][stage];
-      cur_tile = info.w >> 3;
+      cur_tile = info.w >> (kParts + 1);
       if (fresh) {
         fresh = false;
         cur_b = info.x; cur_head = info.y; cur_block = info.z;
@@ -485,23 +521,23 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       __syncwarp();
       const uint8_t* keys_at = ring + (warp * kStages + stage) * Cfg::kStageBytes;
       const uint8_t* values_at = keys_at + Cfg::kCodeBytes + Cfg::kPairBytes;
-      const int first = cur_tile * kKv4Tile;
+      const int first = cur_tile * kTile;
       // not whole: a tile with tokens behind the last one that some row sees, or on a page that could not be followed
-      const bool whole = first + kKv4Tile <= least && (info.w & 3) == 3;
+      const bool whole = first + kTile <= least && (info.w & ((1 << kParts) - 1)) == (1 << kParts) - 1;
       auto usable = [&](int t) { return (info.w >> (t >> 4)) & 1; };
 
       // S^T = K Q^T, in units of key scale * query unit
-      float s[2][kQ][4], top[kQ][2], vscale[2][2];
+      float s[kParts][kQ][4], top[kQ][2], vscale[kParts][2];
 #pragma unroll
       for (int n = 0; n < kQ; ++n) top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < kParts; ++mt) {
         int high[kQ][4], low[kQ][4];
         const int t0 = 16 * mt + turned;
 #pragma unroll
         for (int j = 0; j < kKWords; j += kLoad) {
           uint32_t wa[kLoad], wb[kLoad];
-          const uint8_t* at = keys_at + t0 * (kDim / 2) + 4 * (kLoad * c + j * 4);
+          const uint8_t* at = keys_at + 16 * mt * (kDim / 2) + (key_at ^ 16 * j);   // j = 4: the row's second half
           lds_words(at, wa);
           lds_words(at + 8 * (kDim / 2), wb);
 #pragma unroll
@@ -538,7 +574,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       }
       if (!whole) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < kParts; ++mt)
 #pragma unroll
           for (int n = 0; n < kQ; ++n)
 #pragma unroll
@@ -548,13 +584,15 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
             }
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < kParts; ++mt)
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) top[n][j % 2] = fmaxf(top[n][j % 2], s[mt][n][j]);
-      const float tile_scale = __uint_as_float(__reduce_max_sync(
-          0xffffffffu, __float_as_uint(fmaxf(fmaxf(vscale[0][0], vscale[0][1]), fmaxf(vscale[1][0], vscale[1][1])))));
+      float lane_scale = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < kParts; ++mt) lane_scale = fmaxf(lane_scale, fmaxf(vscale[mt][0], vscale[mt][1]));
+      const float tile_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lane_scale)));
       bool grows = tile_scale > most_scale;
 #pragma unroll
       for (int n = 0; n < kQ; ++n)
@@ -592,14 +630,14 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
           }
       }
       // weights, times the values' scales, transposed into the second product's operand
-      uint32_t w[2][kQ][2];
+      uint32_t w[kParts][kQ][2];
       float base[kQ][2];
 #pragma unroll
       for (int n = 0; n < kQ; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) base[n][e] = m[n][e] == -INFINITY ? 0.f : -m[n][e];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < kParts; ++mt) {
         const float scale[2] = {vscale[mt][0] * value_unit, vscale[mt][1] * value_unit};
 #pragma unroll
         for (int n = 0; n < kQ; ++n) {
@@ -616,7 +654,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       }
       // O^T += V^T P^T
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int mt = 0; mt < kParts; ++mt) {
         uint32_t minus_low[2], minus_high[2], v[4][kVWords];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -627,8 +665,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
           asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(zeros) : "r"(0x43004300u));
           minus_low[r] = (zeros & 0x000f000fu) | 0xe400e400u;
           asm("add.rn.f16x2 %0, %1, %2;" : "=r"(minus_high[r]) : "r"(minus_low[r]), "r"(0x63806380u));   // + 960
-          lds_words(values_at + ta * (kDim / 2) + 4 * kVWords * g, v[2 * r]);
-          lds_words(values_at + tb * (kDim / 2) + 4 * kVWords * g, v[2 * r + 1]);
+          lds_words(values_at + (16 * mt + 8 * r) * (kDim / 2) + even_at, v[2 * r]);
+          lds_words(values_at + (16 * mt + 8 * r) * (kDim / 2) + odd_at, v[2 * r + 1]);
         }
 #pragma unroll
         for (int k = 0; k < kVWords; ++k) {
@@ -653,7 +691,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     if (it + kStages < count) issue(stage);
     copies_commit();
     if (++stage == kStages) stage = 0;
-    if (info.w & 4) {                                    // the last tile of these rows
+    if (info.w >> kParts & 1) {                          // the last tile of these rows
       add_sums();
       if (first_tile == 0) {
         const float unit = 1.f / value_unit;
@@ -690,7 +728,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     add_sums();
     write_piece(2 * warp + 1, reinterpret_cast<float*>(ring + warp * kStages * Cfg::kStageBytes));
     if (lane == 0)
-      pieces[2 * warp + 1] = Kv4Piece{2, first_tile == 0, range + count - 1 - cur_tile, static_cast<unsigned>(kv4_block_tiles(cur_keys)),
+      pieces[2 * warp + 1] = Kv4Piece{2, first_tile == 0, range + count - 1 - cur_tile, static_cast<unsigned>(kv4_block_tiles<kTile>(cur_keys)),
                                       cur_start, cur_block * kRows, min(kRows, cur_rows - cur_block * kRows), cur_head};
   }
   __syncthreads();
