@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   const int page = 1 << p.page_shift;
   const unsigned block_bytes = page * (kDim / 2 + 4), page_bytes = block_bytes * kKv4Side * p.kv_heads;   // at most 70 MB
   const uint32_t ring_base = smem_u32(ring) + warp * kStages * Cfg::kStageBytes;
-  const bool small_page = page < kTile;                  // a tile touches several pages
+  const bool small_page = page % kTile != 0;             // a tile may touch several pages
   constexpr int kRowPieces = kDim / 32;                  // 16-byte pieces of a code row
   constexpr int kCopies = kRowPieces / 2, kPerCopy = 32 / kRowPieces;          // copies for a part's codes, rows a copy covers
   constexpr int kValues = Cfg::kCodeBytes + Cfg::kPairBytes;
@@ -531,34 +531,42 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
 #pragma unroll
       for (int n = 0; n < kQ; ++n) top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
-      for (int mt = 0; mt < kParts; ++mt) {
-        int high[kQ][4], low[kQ][4];
-        const int t0 = 16 * mt + turned;
+      for (int m2 = 0; m2 < kParts; m2 += 2) {
+        int high[2][kQ][4], low[2][kQ][4];
 #pragma unroll
         for (int j = 0; j < kKWords; j += kLoad) {
-          uint32_t wa[kLoad], wb[kLoad];
-          const uint8_t* at = keys_at + 16 * mt * (kDim / 2) + (key_at ^ 16 * j);   // j = 4: the row's second half
-          lds_words(at, wa);
-          lds_words(at + 8 * (kDim / 2), wb);
+          uint32_t wa[2][kLoad], wb[2][kLoad];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+          const uint8_t* at = keys_at + 16 * (m2 + u) * (kDim / 2) + (key_at ^ 16 * j);
+          lds_words(at, wa[u]);
+          lds_words(at + 8 * (kDim / 2), wb[u]);
+          }
 #pragma unroll
           for (int k = 0; k < kLoad; ++k) {
-            const uint32_t a0 = wa[k] & 0x0f0f0f0fu, a1 = wb[k] & 0x0f0f0f0fu, a2 = (wa[k] >> 4) & 0x0f0f0f0fu, a3 = (wb[k] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t a0 = wa[u][k] & 0x0f0f0f0fu, a1 = wb[u][k] & 0x0f0f0f0fu, a2 = (wa[u][k] >> 4) & 0x0f0f0f0fu, a3 = (wb[u][k] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
             for (int n = 0; n < kQ; ++n) {
               const uint32_t(&d)[4] = q[j + k][n];
               if (j + k == 0) {
-                mma_u8s8_first(high[n], a0, a1, a2, a3, d[0], d[1]);
-                mma_u8s8_first(low[n], a0, a1, a2, a3, d[2], d[3]);
+                mma_u8s8_first(high[u][n], a0, a1, a2, a3, d[0], d[1]);
+                mma_u8s8_first(low[u][n], a0, a1, a2, a3, d[2], d[3]);
               } else {
-                mma_u8s8(high[n], a0, a1, a2, a3, d[0], d[1]);
-                mma_u8s8(low[n], a0, a1, a2, a3, d[2], d[3]);
+                mma_u8s8(high[u][n], a0, a1, a2, a3, d[0], d[1]);
+                mma_u8s8(low[u][n], a0, a1, a2, a3, d[2], d[3]);
               }
             }
           }
+          }
         }
 #pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int t = t0 + 8 * r;
+          const int mt = m2 + u;
+          const int t = 16 * mt + turned + 8 * r;
           const uint32_t key_pair = lds32(keys_at + Cfg::kCodeBytes + 4 * t);
           vscale[mt][r] = bf16_lo(lds32(values_at + Cfg::kCodeBytes + 4 * t));
           const float kscale = bf16_lo(key_pair);
@@ -566,10 +574,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
 #pragma unroll
           for (int n = 0; n < kQ; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // below 2^28: exact
-              s[mt][n][2 * r + e] = static_cast<float>(high[n][2 * r + e] * 256 + low[n][2 * r + e] - zero * qsum[n][e]) * kscale;
-            }
+            for (int e = 0; e < 2; ++e)
+              s[mt][n][2 * r + e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]) * kscale;
         }
       }
       if (!whole) {
