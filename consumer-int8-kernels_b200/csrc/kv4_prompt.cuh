@@ -71,14 +71,29 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint32_t b, 
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
+// 16 rows x 64 columns: lane 4 g + c holds columns 8 i + 2 c and 8 i + 2 c + 1 of row g in v[4 i], v[4 i + 1] and of row
+// g + 8 in v[4 i + 2], v[4 i + 3].
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
-      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_16x64(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+// 16 rows x 32 columns: column 4 i + c of row g in v[2 i], of row g + 8 in v[2 i + 1].
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -145,6 +160,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
   __shared__ __align__(16) float scale_k[kKv4ScaleSlots][kKeys], scale_v[kKv4ScaleSlots][kKeys];
   __shared__ uint32_t hidden[kKv4MarkSlots][kKeys / 32];   // keys of the tile on a page that could not be followed
   __shared__ int any_hidden[kKv4MarkSlots];
+  __shared__ float row_max[2][128], row_sum[2][128];
   __shared__ uint32_t tmem_base;
   __shared__ int abort_flag, tile_info[2];
   const Kv4AttendParams& p = params.a;
@@ -246,63 +262,89 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bar_q));
       }
-      const int token = p.group.quotient(row);
-      const int limit = row < all_rows ? max(0, seq.keys - seq.rows + token + 1) : 0;
-      const int least = __reduce_min_sync(0xffffffffu, limit);
-      const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16;
+      constexpr int kRuns = kKeys / 64;
+      // A warp's 32 rows as TMEM hands them out: lane 4 g + c works on rows g, g + 8, g + 16, g + 24 and on the keys 8 i + 2 c
+      // and 8 i + 2 c + 1 of each. A lane then needs the scales of 16 keys of 64; with a whole row to a lane the scales'
+      // broadcasts took as much of the shared memory's bandwidth as the MMAs' operands.
+      const int g = lane / 4, c = lane % 4;
+      int limit[4], least = 0x7fffffff;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int q_row = first_row + 128 * t + 32 * (warp % 4) + 8 * r + g;
+        limit[r] = q_row < all_rows ? max(0, seq.keys - seq.rows + p.group.quotient(q_row) + 1) : 0;
+        least = min(least, limit[r]);
+      }
+      least = __reduce_min_sync(0xffffffffu, least);
+      const uint32_t lanes = static_cast<uint32_t>(warp % 4 * 32) << 16, half = 16u << 16;   // rows 16 .. 31 of the warp
       const uint32_t output = tmem + lanes + kOutputColumn + t * kDim;
-      float m = -INFINITY;
-      float2 sum2 = make_float2(0.f, 0.f);
+      float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float2 sum2[4] = {};
       bool fine = true;
       for (int j = 0; j < tiles && fine; ++j) {
         const int buffer = kQTiles == 2 ? t : j & 1;
         const uint32_t scores = tmem + lanes + 128 * buffer;
         const int slot = j % kKv4ScaleSlots, slot_parity = j / kKv4ScaleSlots & 1;
-        const int parity = kQTiles == 2 ? j & 1 : j >> 1 & 1;
-        fine = warp_wait(&bar_s[buffer], parity, &abort_flag) && warp_wait(&bar_scale_k[slot], slot_parity, &abort_flag);
+        fine = warp_wait(&bar_s[buffer], kQTiles == 2 ? j & 1 : j >> 1 & 1, &abort_flag) && warp_wait(&bar_scale_k[slot], slot_parity, &abort_flag);
         if (!fine) break;
         tcgen05_fence_after();
-        uint32_t s[kKeys / 32][32];
+        uint32_t s[kRuns][2][32];                        // [64 keys][rows g and g + 8, rows g + 16 and g + 24]
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(scores + 32 * c, s[c]);
-#pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) tmem_ld_wait_for(s[c]);
-        const int first_key = (begin + j) * kKeys;
-        const bool masked = first_key + kKeys > least || any_hidden[j % kKv4MarkSlots];
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k = *reinterpret_cast<const float4*>(&scale_k[slot][32 * c + i]);
-            const float2 lo = __fmul2_rn(make_float2(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), make_float2(k.x, k.y));
-            const float2 hi = __fmul2_rn(make_float2(__uint_as_float(s[c][i + 2]), __uint_as_float(s[c][i + 3])), make_float2(k.z, k.w));
-            s[c][i] = __float_as_uint(lo.x);
-            s[c][i + 1] = __float_as_uint(lo.y);
-            s[c][i + 2] = __float_as_uint(hi.x);
-            s[c][i + 3] = __float_as_uint(hi.y);
-          }
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c) {
-            const int seen = min(32, max(0, limit - first_key - 32 * c));
-            const uint32_t shown = (seen == 32 ? ~0u : (1u << seen) - 1) & ~hidden[j % kKv4MarkSlots][c];
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(shown >> i & 1)) s[c][i] = 0xff800000u;
-          }
+        for (int h = 0; h < kRuns; ++h) {
+          tmem_ld_16x64(scores + 64 * h, s[h][0]);
+          tmem_ld_16x64(scores + 64 * h + half, s[h][1]);
         }
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c)
+        for (int h = 0; h < kRuns; ++h) {
+          tmem_ld_wait_for(s[h][0]);
+          tmem_ld_wait_for(s[h][1]);
+        }
+        const int first_key = (begin + j) * kKeys;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-        if (__any_sync(0xffffffffu, most > m + 8.f)) {
-          const float next = fmaxf(m, most);
-          const float keep = next == -INFINITY ? 1.f : kv4_exp2(m - next);
-          m = next;
-          sum2.x *= keep;
-          sum2.y *= keep;
+        for (int i = 0; i < 8 * kRuns; ++i) {
+          const float2 k = *reinterpret_cast<const float2*>(&scale_k[slot][8 * i + 2 * c]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uint32_t* at = &s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1)];
+            const float2 x = __fmul2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), k);
+            at[0] = __float_as_uint(x.x);
+            at[1] = __float_as_uint(x.y);
+          }
+        }
+        if (first_key + kKeys > least || any_hidden[j % kKv4MarkSlots]) {
+#pragma unroll
+          for (int i = 0; i < 8 * kRuns; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = 8 * i + 2 * c + e;
+              const bool marked = hidden[j % kKv4MarkSlots][key / 32] >> (key % 32) & 1;
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (marked || first_key + key >= limit[r]) s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1) + e] = 0xff800000u;
+            }
+        }
+        bool grows = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int i = 0; i < 8 * kRuns; ++i) {
+            const uint32_t* at = &s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1)];
+            top[r] = max3(top[r], __uint_as_float(at[0]), __uint_as_float(at[1]));
+          }
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.scale_log2;
+          grows |= top[r] > m[r] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+          float keep[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float next = fmaxf(m[r], top[r]);
+            keep[r] = next == -INFINITY ? 1.f : kv4_exp2(m[r] - next);
+            m[r] = next;
+            sum2[r].x *= keep[r];
+            sum2[r].y *= keep[r];
+          }
           if (j > 0) {
             // Two query tiles: these scores were issued behind the product that last wrote the output, which is
             // complete. One: that product may still be running.
@@ -312,51 +354,67 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
               tcgen05_fence_after();
             }
 #pragma unroll 1
-            for (int c = 0; c < kDim; c += 32) {
+            for (int part = 0; part < 2 * (kDim / 64); ++part) {
+              const uint32_t at = output + 64 * (part / 2) + (part & 1 ? half : 0);
+              const float low = part & 1 ? keep[2] : keep[0], high = part & 1 ? keep[3] : keep[1];
               uint32_t o[32];
-              tmem_ld_32x32(output + c, o);
+              tmem_ld_16x64(at, o);
               tmem_ld_wait_for(o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-              tmem_st_32x32(output + c, o);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * (i & 2 ? high : low));
+              tmem_st_16x64(at, o);
             }
           }
         }
         fine = warp_wait(&bar_scale_v[slot], slot_parity, &abort_flag);
         if (!fine) break;
-        const float base = m == -INFINITY ? 0.f : -m;
-        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), base2 = make_float2(base, base);
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+        float2 base2[4];
 #pragma unroll
-        for (int h = 0; h < kKeys / 64; ++h) {
-          uint32_t packed[32];
+        for (int r = 0; r < 4; ++r) base2[r].x = base2[r].y = m[r] == -INFINITY ? 0.f : -m[r];
 #pragma unroll
-          for (int i = 0; i < 64; i += 4) {
-            uint32_t(&from)[32] = s[2 * h + i / 32];
-            const float4 v = *reinterpret_cast<const float4*>(&scale_v[slot][64 * h + i]);
-            float2 x = __ffma2_rn(make_float2(__uint_as_float(from[i % 32]), __uint_as_float(from[i % 32 + 1])), scale2, base2);
-            float2 y = __ffma2_rn(make_float2(__uint_as_float(from[i % 32 + 2]), __uint_as_float(from[i % 32 + 3])), scale2, base2);
-            x = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
-            y = make_float2(kv4_exp2(y.x), kv4_exp2(y.y));
-            sum2 = __fadd2_rn(sum2, x);
-            sum2 = __fadd2_rn(sum2, y);
-            x = __fmul2_rn(x, make_float2(v.x, v.y));
-            y = __fmul2_rn(y, make_float2(v.z, v.w));
-            packed[i / 2] = pack2(x.x, x.y);
-            packed[i / 2 + 1] = pack2(y.x, y.y);
+        for (int h = 0; h < kRuns; ++h) {
+          uint32_t packed[2][16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 v = *reinterpret_cast<const float2*>(&scale_v[slot][64 * h + 8 * i + 2 * c]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t* at = &s[h][r / 2][4 * i + 2 * (r & 1)];
+              float2 x = __ffma2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), scale2, base2[r]);
+              x = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
+              sum2[r] = __fadd2_rn(sum2[r], x);
+              x = __fmul2_rn(x, v);
+              packed[r / 2][2 * i + (r & 1)] = pack2(x.x, x.y);
+            }
           }
-          tmem_st_32x32(scores + 32 * h, packed);
+          tmem_st_16x32(scores + 32 * h, packed[0]);
+          tmem_st_16x32(scores + 32 * h + half, packed[1]);
           tmem_st_wait();
           tcgen05_fence_before();
           mbar_arrive(smem_u32(&bar_p[buffer][h]));      // the product may begin on the first half of the keys
         }
       }
+      // the rows' maxima and sums, for the lanes that hold them in the output's layout (one row to a lane)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float all = sum2[r].x + sum2[r].y;
+        all += __shfl_xor_sync(0xffffffffu, all, 1);
+        all += __shfl_xor_sync(0xffffffffu, all, 2);
+        if (c == 0) {
+          row_max[t][32 * (warp % 4) + 8 * r + g] = m[r];
+          row_sum[t][32 * (warp % 4) + 8 * r + g] = all;
+        }
+      }
+      __syncwarp();
+      const int token = p.group.quotient(row);
+      const float sum = row_sum[t][row_in_tile];
       // ---- output
       if (fine && tiles > 0) fine = warp_wait(&bar_done[t], 0, &abort_flag);
       tcgen05_fence_after();
-      const float sum = sum2.x + sum2.y;
       if (params.partial) {
         float* slot = params.partial + (((static_cast<int64_t>(blockIdx.x) * p.kv_heads + head) * params.splits + split) * Cfg::kRows + 128 * t) * (kDim + 2);
-        slot[row_in_tile] = m;                             // [128 maxima][128 sums][128 outputs]
+        slot[row_in_tile] = row_max[t][row_in_tile];       // [128 maxima][128 sums][128 outputs]
         slot[128 + row_in_tile] = sum;
         float* dst = slot + 256 + row_in_tile * kDim;
         if (tiles > 0 && fine) {
