@@ -78,7 +78,8 @@ def values(cache, dim):
 
 
 def attention(q, cache, block_table, q_starts, kv_lens, scale):
-    """(out FP64 [tokens, q_heads, dim], the bound's weights: sum of p * |v| and sum of |q| * step * scale)."""
+    """(out FP64 [tokens, q_heads, dim], the bound's weights: sum of p * |v|, and the largest score a row could have,
+    dim * 15 steps * max |q| * scale)."""
     tokens, q_heads, dim = q.shape
     held = values(cache, dim)
     _, pairs = rows(cache, dim)
@@ -103,5 +104,5 @@ def attention(q, cache, block_table, q_starts, kv_lens, scale):
                 p = (k @ row * scale).softmax(0)
                 out[start + i, h] = p @ v
                 spread[start + i, h] = p @ v.abs()
-                reach[start + i, h] = row.abs().sum() * step[h * kv_heads // q_heads, seen].max() * scale
+                reach[start + i, h] = row.abs().max() * 15 * dim * step[h * kv_heads // q_heads, seen].max() * scale
     return out, spread, reach

@@ -1,10 +1,13 @@
 """kv4_attention against the CPU restatement in 64 bits.
 
-Bound of an output component y = sum of p_j v_j: one BF16 rounding of y (half a step, 2^-8), one BF16 rounding of every
-weight (2^-8 of the sum of p_j |v_j|, FP32 sums beside it), and the scores' FP32 errors. A score is
-step * scale * (sum of q_i c_i - zero * sum of q_i) with codes that may carry an offset of 128, accumulated by the matrix
-instructions over at most 16 steps and 8 further FP32 operations, each off by at most 2^-23 of the largest partial sum,
-(128 + 15) * sum |q_i|; a score that is off by d moves every weight by at most a factor exp(2 d)."""
+Bound of an output component y = sum of p_j v_j, with R = dim * 15 steps * max |q| * scale, the largest score of the row:
+  one BF16 rounding of y: half a step, 2^-8 |y|;
+  one rounding of every weight times its value's scale, to BF16 (prompts) or FP16 (generated tokens, 2^-11): 2^-8 of the sum
+  of p_j |v_j|, FP32 sums and exponentials (2^-22) beside it: 5 % more;
+  a score's error d, which moves every weight by at most a factor exp(2 d) (its own and the sum's). Generated tokens: a query
+  component is a multiple of max |q| / 32639, off by at most 2^-16 of max |q| (half of 1 / 32639, rounded up); the sum of
+  products with codes less zero points is exact, so d <= 2^-16 R and a few FP32 roundings, 2^-21 R. Prompts: the products
+  are exact, accumulated over at most 16 steps with 2^-23 of the largest partial sum each: below 2^-18 R."""
 import pytest
 import torch
 
@@ -15,7 +18,7 @@ pytestmark = pytest.mark.gpu
 
 
 def tolerance(want, spread, reach):
-    score = 24 * 2.0 ** -23 * 143 * reach
+    score = (2.0 ** -16 + 2.0 ** -21) * reach
     return 2.0 ** -8 * want.abs() + (1.05 * 2.0 ** -8 + torch.expm1(2 * score)) * spread
 
 
