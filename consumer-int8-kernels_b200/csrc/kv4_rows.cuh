@@ -58,7 +58,7 @@ __device__ __forceinline__ float approximate_reciprocal(float x) {
 }
 __device__ __forceinline__ Kv4Code kv4_code_of(float low, float high) {
   Kv4Code c;
-  const float step = __fdiv_rn(__fsub_rn(high, low), 15.f);
+  const float step = __fmul_rn(__fsub_rn(high, low), 1.f / 15.f);
   c.scale = fmaxf(__bfloat162float(__float2bfloat16_rn(step)), __bfloat162float(__float2bfloat16_rn(1e-20f)));
   c.inverse = approximate_reciprocal(c.scale);
   float rounded = __fsub_rn(__fmaf_rn(-low, c.inverse, kRoundMagic), kRoundMagic);

@@ -244,8 +244,9 @@ int ci8_qk_norm_rope(const void* q, long long q_stride, const void* k, long long
                      float weight_offset, int adjacent, ci8_stream_t stream);
 
 /* Appends keys and values to the cache: keys are rotated as above (not when cos_sin is NULL), then every key and
- * value head is encoded: low = min(x, 0), high = max(x, 0) over the head, scale = bf16((high - low) / 15), at least
- * 1e-20, zero = rint(-low / scale), code = clamp(rint(x / scale) + zero, 0, 15), IEEE divisions, halves to even.
+ * value head is encoded: low = min(x, 0), high = max(x, 0) over the head, scale = bf16((high - low) * (1/15)), at
+ * least 1e-20, zero = rint(-low / scale), code = clamp(rint(x / scale) + zero, 0, 15): FP32, one IEEE operation at a time,
+ * halves to even.
  * NaN counts as 0, infinities as +-8.5e37. q (NULL: none) is rotated into q_out in the same launch. slots INT64
  * [tokens]: where each token goes; a negative slot is not stored (padding; its query is still rotated), nor is one
  * beyond the cache or a token with a bad position (status bit 3). Slots that are stored must differ: two tokens

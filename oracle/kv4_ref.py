@@ -42,7 +42,8 @@ def encode(x):
     assert x.dtype == torch.float32
     x = torch.nan_to_num(x, nan=0.0, posinf=8.5e37, neginf=-8.5e37).clamp(-8.5e37, 8.5e37)
     low, high = x.amin(-1).clamp(max=0), x.amax(-1).clamp(min=0)
-    scale = torch.maximum(((high - low) / 15).bfloat16(), torch.tensor(1e-20).bfloat16())
+    step = (high - low) * torch.tensor(1.0 / 15.0)         # the FP32 number next to 1 / 15
+    scale = torch.maximum(step.bfloat16(), torch.tensor(1e-20).bfloat16())
     s = scale.float()
     zero = torch.round(-low / s).clamp(0, 15) + 0.0        # a whole number: never minus zero
     codes = (torch.round(x / s[..., None]) + zero[..., None]).clamp(0, 15)
