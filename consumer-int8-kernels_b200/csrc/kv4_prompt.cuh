@@ -5,12 +5,20 @@
 // hold the scores and outputs of no more). It walks the keys in tiles of 128 (64 for dim 256):
 //   unpack warps   codes from global memory (a half-step ahead, in registers) -> BF16 code - zero, exact small integers,
 //                  into the 128-byte-swizzled operand tiles; scales beside them as FP32
-//   MMA warp       S = Q K^T (both from shared memory), O += P V (P from TMEM)
-//   softmax warps  one thread per row: S * key scale, running maximum and sum, weights * value scale rounded to BF16
+//   MMA warp       S = Q K^T (Q from TMEM where it has room, from shared memory for dim 128), O += P V (P from TMEM)
+//   softmax warps  32 rows each: S * key scale, running maximum and sum, weights * value scale rounded to BF16
 //                  into the columns of S. The output is scaled only when a row's maximum has grown by more than 2^8.
 // The components of a word come out of the unpacking as 0 4 1 5 2 6 3 7; the queries are stored in that order and the
-// output is put back. The tensor pipe needs 4 * dim * 256 / 8192 cycles per key, the exponentials 256 / 16: equal at
-// dim 128, so both have to run all the time; the two query tiles take turns on either.
+// output is put back.
+//
+// What bounds it is not the tensor pipe (a third busy) but what feeds it. Dim 256, where a tile of keys serves 128 rows
+// only: the unpacking (11 instructions and one 16-byte store for eight components), ahead of the shared memory's bandwidth.
+// Dim 128: the chain scores -> softmax -> product -> next scores of each query tile, of which two run at a time, with 39 %
+// of the cycles taken by the exponentials. Measured (32 query heads and 8 key heads of 128, 8192 new tokens): 775 us,
+// 710 TFLOP/s; 24 and 4 heads of 256, 4096 tokens behind 4096: 779 us, 794 TFLOP/s, where queries in shared memory and lanes
+// that load from eight rows at a time took 1020; 32 and 8 heads of 64, 8192 tokens: 629 us. Tried and slower: tiles of 64 keys
+// with two score buffers for dim 128 (792), the tiles of keys dealt to two softmax warpgroups in turn (831; dim 256 880
+// against 876 then), four unpacking warpgroups for dim 256 (917 against 876), more registers for the softmax (782 to 821).
 #pragma once
 #include "kv4_attention.cuh"
 
@@ -25,8 +33,13 @@ struct Kv4PromptConfig {
   static constexpr int kThreads = 512;                   // softmax, unpack and MMA warpgroups
   static constexpr int kQBytes = 128 * kDim * 2;
   static constexpr int kTileBytes = kKeys * kDim * 2;
-  static constexpr int kStages = 2;
-  static constexpr int kSmemBytes = kQTiles * kQBytes + 2 * kStages * kTileBytes + 1024;
+  // TMEM columns: two score buffers, the outputs from 256 on, and where they leave room the queries, which the score
+  // products then need not read from shared memory for every tile of keys.
+  static constexpr bool kQInTmem = kDim != 128;
+  static constexpr int kScoreColumns = kDim == 256 ? 64 : 128;
+  static constexpr int kQColumn = kDim == 256 ? 128 : 384;
+  static constexpr int kStages = kDim == 256 ? 3 : 2;
+  static constexpr int kSmemBytes = (kQInTmem ? 0 : kQTiles * kQBytes) + 2 * kStages * kTileBytes + 1024;
   // registers per thread after the hand-over; together 512 * 128
   static constexpr int kSoftmaxRegs = 192;
   static constexpr int kUnpackRegs = kDim == 256 ? 120 : 88;
@@ -42,11 +55,12 @@ struct Kv4PromptParams {
   int most_rows;              // sequences with no more query rows than this belong to another kernel
 };
 
-// Scales are read by the softmax warps, up to two tiles behind the unpacking: the values of tile j + 2 are not unpacked
-// before the second product of tile j, whose weights come after its scales were read. So tile j + 4 may take tile j's slot,
-// and the marks of tile j + 4 can be cleared while tile j's are being set.
-constexpr int kKv4ScaleSlots = 4;
-constexpr int kKv4MarkSlots = 8;
+// Scales are read by the softmax warps, some tiles behind the unpacking: the keys of tile j + kStages are unpacked when the
+// scores of tile j are complete, and those were issued behind a product with the weights of tile j - 2 (or j - 1), whose
+// scales were read then. So tile j may take the slot of tile j - 8 as long as kStages + 2 <= 8; the marks of tile j + 8 are
+// cleared while those of tile j are set.
+constexpr int kKv4ScaleSlots = 8;
+constexpr int kKv4MarkSlots = 2 * kKv4ScaleSlots;
 
 __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, bool b_transposed) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -84,6 +98,14 @@ __device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&v)[32])
 __device__ __forceinline__ void tmem_st_16x64(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+// 32 rows, one to a lane, x 32 columns.
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
@@ -154,6 +176,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
   constexpr int kSegments = kDim / 64;                   // of 64 components, 128 bytes a row
   constexpr int kSoftmaxGroups = kQTiles;
   constexpr uint32_t kOutputColumn = 256;
+  static_assert(kStages + 2 <= kKv4ScaleSlots, "a slot's scales have been read when it is filled again");
   extern __shared__ uint8_t dynamic_smem[];
   __shared__ __align__(8) uint64_t bar_q, bar_s[2], bar_p[2][2], bar_done[2], bar_k[kStages], bar_k_free[kStages], bar_v[kStages], bar_v_free[kStages];
   __shared__ __align__(8) uint64_t bar_scale_k[kKv4ScaleSlots], bar_scale_v[kKv4ScaleSlots];
@@ -167,7 +190,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
   const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32, warpgroup = warp / 4;
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* const q_smem = smem;
-  uint8_t* const k_smem = smem + kQTiles * Cfg::kQBytes;
+  uint8_t* const k_smem = smem + (Cfg::kQInTmem ? 0 : kQTiles * Cfg::kQBytes);
   uint8_t* const v_smem = k_smem + kStages * Cfg::kTileBytes;
 
   if (warp == 0) {
@@ -231,10 +254,32 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
     const int tiles = end - begin;
 
     if (warpgroup < kSoftmaxGroups) {
-      // ================================================================ softmax: one thread per query row
+      // ================================================================ softmax
       setmaxnreg_inc<Cfg::kSoftmaxRegs>();
       const int t = warpgroup, row_in_tile = thread % 128, row = first_row + 128 * t + row_in_tile;
-      {
+      if constexpr (Cfg::kQInTmem) {
+        // the thread's query row, in the unpacked codes' order
+        const int token = p.group.quotient(row);
+        const uint16_t* src = p.q + (seq.start + token) * p.q_stride + static_cast<int64_t>(head * group + row - token * group) * kDim;
+#pragma unroll 1
+        for (int base = 0; base < kDim; base += 64) {
+          uint4 w[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) w[n] = row < all_rows ? *reinterpret_cast<const uint4*>(src + base + 8 * n) : make_uint4(0, 0, 0, 0);
+          uint32_t x[32];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            x[4 * n] = __byte_perm(w[n].x, w[n].z, 0x5410);
+            x[4 * n + 1] = __byte_perm(w[n].x, w[n].z, 0x7632);
+            x[4 * n + 2] = __byte_perm(w[n].y, w[n].w, 0x5410);
+            x[4 * n + 3] = __byte_perm(w[n].y, w[n].w, 0x7632);
+          }
+          tmem_st_32x32(tmem + (static_cast<uint32_t>(warp % 4 * 32) << 16) + Cfg::kQColumn + (t * kDim + base) / 2, x);
+        }
+        tmem_st_wait();
+        tcgen05_fence_before();
+        mbar_arrive(smem_u32(&bar_q));
+      } else {
         // the tile's queries, in the unpacked codes' order
         constexpr int kPieces = kDim / 8;
         uint8_t* const tile = q_smem + t * Cfg::kQBytes;
@@ -282,36 +327,40 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       bool fine = true;
       for (int j = 0; j < tiles && fine; ++j) {
         const int buffer = kQTiles == 2 ? t : j & 1;
-        const uint32_t scores = tmem + lanes + 128 * buffer;
+        const uint32_t scores = tmem + lanes + Cfg::kScoreColumns * buffer;
         const int slot = j % kKv4ScaleSlots, slot_parity = j / kKv4ScaleSlots & 1;
         fine = warp_wait(&bar_s[buffer], kQTiles == 2 ? j & 1 : j >> 1 & 1, &abort_flag) && warp_wait(&bar_scale_k[slot], slot_parity, &abort_flag);
         if (!fine) break;
         tcgen05_fence_after();
         uint32_t s[kRuns][2][32];                        // [64 keys][rows g and g + 8, rows g + 16 and g + 24]
-#pragma unroll
-        for (int h = 0; h < kRuns; ++h) {
-          tmem_ld_16x64(scores + 64 * h, s[h][0]);
-          tmem_ld_16x64(scores + 64 * h + half, s[h][1]);
-        }
+        const int first_key = (begin + j) * kKeys;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld_16x64(scores, s[0][0]);
+        tmem_ld_16x64(scores + half, s[0][1]);
 #pragma unroll
         for (int h = 0; h < kRuns; ++h) {
           tmem_ld_wait_for(s[h][0]);
           tmem_ld_wait_for(s[h][1]);
-        }
-        const int first_key = (begin + j) * kKeys;
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (h + 1 < kRuns) {                           // the next keys' scores are on their way while these are in work
+            tmem_ld_16x64(scores + 64 * (h + 1), s[h + 1][0]);
+            tmem_ld_16x64(scores + 64 * (h + 1) + half, s[h + 1][1]);
+          }
 #pragma unroll
-        for (int i = 0; i < 8 * kRuns; ++i) {
-          const float2 k = *reinterpret_cast<const float2*>(&scale_k[slot][8 * i + 2 * c]);
+          for (int i = 0; i < 8; ++i) {
+            const float2 k = *reinterpret_cast<const float2*>(&scale_k[slot][64 * h + 8 * i + 2 * c]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            uint32_t* at = &s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1)];
-            const float2 x = __fmul2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), k);
-            at[0] = __float_as_uint(x.x);
-            at[1] = __float_as_uint(x.y);
+            for (int r = 0; r < 4; ++r) {
+              uint32_t* at = &s[h][r / 2][4 * i + 2 * (r & 1)];
+              const float2 x = __fmul2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), k);
+              at[0] = __float_as_uint(x.x);
+              at[1] = __float_as_uint(x.y);
+              top[r] = max3(top[r], x.x, x.y);
+            }
           }
         }
         if (first_key + kKeys > least || any_hidden[j % kKv4MarkSlots]) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top[r] = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 8 * kRuns; ++i)
 #pragma unroll
@@ -319,18 +368,16 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
               const int key = 8 * i + 2 * c + e;
               const bool marked = hidden[j % kKv4MarkSlots][key / 32] >> (key % 32) & 1;
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (marked || first_key + key >= limit[r]) s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1) + e] = 0xff800000u;
+              for (int r = 0; r < 4; ++r) {
+                uint32_t& x = s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1) + e];
+                if (marked || first_key + key >= limit[r]) x = 0xff800000u;
+                top[r] = fmaxf(top[r], __uint_as_float(x));
+              }
             }
         }
         bool grows = false;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-#pragma unroll
-          for (int i = 0; i < 8 * kRuns; ++i) {
-            const uint32_t* at = &s[i / 8][r / 2][4 * (i % 8) + 2 * (r & 1)];
-            top[r] = max3(top[r], __uint_as_float(at[0]), __uint_as_float(at[1]));
-          }
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.scale_log2;
           grows |= top[r] > m[r] + 8.f;
@@ -460,54 +507,44 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       // One group unpacks keys and values in turn; two groups take one each.
       const int side_first = Cfg::kUnpackGroups == 2 ? warpgroup - kSoftmaxGroups : 0;
       constexpr int kSteps = Cfg::kUnpackGroups == 2 ? 1 : 2;          // half-steps (sides) per tile of keys
-      // Lane mapping: eight neighbouring lanes take eight rows of one piece of 16 code bytes (conflict-free stores), the
-      // four such octets the pieces (dim 128), half the pieces (256), or the pieces of two runs of rows (64).
-      constexpr int kPasses = kDim == 64 ? 2 : kDim == 128 ? 4 : 2;
-      constexpr int kLoads = kDim == 256 ? 2 : 1;                      // pieces of a row a lane takes
-      constexpr int kPassRows = kKeys / kPasses;
-      const int octet = lane / 8;
-      const int lane_row = (kDim == 64 ? 16 * (warp % 4) + 8 * (octet / 2) : 8 * (warp % 4)) + lane % 8;
-      const int lane_piece = kDim == 64 ? octet % 2 : octet;
+      // Eight neighbouring lanes load pieces of 16 code bytes and store 16 bytes of components together. Both want different
+      // banks: four rows of two pieces for dim 64 and 128, and for dim 256 one row, whose words the lanes then store in an
+      // order of their own (word ^ turn), at the cost of the selections.
+      constexpr int kPieces = kDim / 32, kPassRows = 128 / kPieces, kPasses = kKeys / kPassRows;
+      const int lane_row = kPassRows / 4 * (warp % 4) + (kDim == 128 ? lane / 2 % 4 + lane / 16 * 4 : lane / kPieces);
+      const int lane_piece = kDim == 128 ? lane % 2 + lane / 8 % 2 * 2 : lane % kPieces;
+      const int turn = kDim == 256 ? lane_piece / 2 : 0;
       const int page = 1 << p.page_shift;
       const unsigned block_bytes = page * (kDim / 2 + 4), page_bytes = block_bytes * kKv4Side * p.kv_heads;   // at most 70 MB
       const uint8_t* const head_src = p.cache + static_cast<uint64_t>(head) * block_bytes;
       const int32_t* const table = p.block_table + static_cast<int64_t>(b) * p.width;
-      // page numbers of the keys ahead: 32 in the lanes and the next 32 behind them
-      int window_first = begin * kKeys >> p.page_shift;
-      auto load_window = [&](int from) {
-        const int64_t index = static_cast<int64_t>(from) + lane;
-        return (index << p.page_shift) < keys ? table[index] : -1;
-      };
-      int window = load_window(window_first), window_next = load_window(window_first + 32);
-      uint4 codes[kPasses][kLoads];
+      // A run of 16 keys lies on one page, and a warp's rows of a pass in one run. Page numbers are loaded a tile ahead of the
+      // codes: lane l holds the one of the tile's run l.
+      constexpr int kRunsOfTile = kKeys / 16;
+      auto load_ids = [&](int j) { return table[min((begin + j) * kKeys + 16 * lane, keys - 1) >> p.page_shift]; };
+      const int lane_code = lane_row % 16 * (kDim / 2) + 16 * lane_piece, lane_pair = page * (kDim / 2) + 4 * (lane_row % 16);
+      int ids = -1, ids_ahead = tiles > 0 ? load_ids(0) : -1;
+      uint4 codes[kPasses];
       uint32_t pairs[kPasses];                           // (nothing may touch what is loaded before the next half-step)
-      uint32_t marks = 0, live = 0;                      // passes whose key lies on a page that cannot be followed, whose key is there
+      uint32_t live = 0, marks = 0;                      // runs whose keys are there, that lie on a page that cannot be followed
       auto load = [&](int step) {
-        const int tile = begin + step / kSteps, side = kSteps == 2 ? step & 1 : side_first;
+        const int j = step / kSteps, side = kSteps == 2 ? step & 1 : side_first, first = (begin + j) * kKeys;
         const uint8_t* const side_src = head_src + side * p.kv_heads * block_bytes;
-        marks = live = 0;
-        while ((((tile + 1) * kKeys - 1) >> p.page_shift) - window_first >= 32 + 32) {
-          window_first += 32;
-          window = window_next;
-          window_next = load_window(window_first + 32);
+        if (kSteps == 1 || side == 0) {
+          ids = ids_ahead;
+          ids_ahead = load_ids(j + 1);
         }
+        const bool wanted = lane < kRunsOfTile && first + 16 * lane < keys, good = wanted && static_cast<unsigned>(ids) < static_cast<unsigned>(p.pages);
+        live = __ballot_sync(0xffffffffu, good);
+        marks = __ballot_sync(0xffffffffu, wanted && !good);
+        const unsigned id = good ? ids : 0u;             // a run that is not there reads the cache's first page and is made zero when it is used
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
-          const int key = tile * kKeys + kPassRows * i + lane_row;
-          const int index = (key >> p.page_shift) - window_first;
-          const int low = __shfl_sync(0xffffffffu, window, index & 31), high = __shfl_sync(0xffffffffu, window_next, index & 31);
-          const unsigned id = index < 32 ? low : high;
-          const bool wanted = key < keys, good = wanted && id < static_cast<unsigned>(p.pages);
-          marks |= wanted && !good ? 1u << i : 0u;
-          live |= good ? 1u << i : 0u;
-          // a key that is not there reads the cache's first page instead and is made zero when it is used
-          const uint8_t* src = side_src + static_cast<uint64_t>(good ? id : 0u) * page_bytes;
-          const int at = key & (page - 1);
+          const int run = (kPassRows * i + lane_row) / 16, at = (first + 16 * run) & (page - 1);
+          const uint8_t* src = side_src + static_cast<uint64_t>(__shfl_sync(0xffffffffu, id, run)) * page_bytes;
           if (p.pages > 0) {
-            pairs[i] = __ldcg(reinterpret_cast<const unsigned*>(src + page * (kDim / 2) + 4 * at));
-#pragma unroll
-            for (int n = 0; n < kLoads; ++n)
-              codes[i][n] = __ldcg(reinterpret_cast<const uint4*>(src + at * (kDim / 2) + 16 * (lane_piece + 4 * n)));
+            pairs[i] = __ldcg(reinterpret_cast<const unsigned*>(src + (4 * at + lane_pair)));
+            codes[i] = __ldcg(reinterpret_cast<const uint4*>(src + (at * (kDim / 2) + lane_code)));
           }
         }
       };
@@ -519,25 +556,24 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         const int stage = j % kStages, slot = j % kKv4ScaleSlots;
         uint64_t* const full = side ? bar_v : bar_k;
         uint64_t* const empty = side ? bar_v_free : bar_k_free;
-        uint4 now[kPasses][kLoads];
+        uint4 now[kPasses];
         uint32_t now_pairs[kPasses];
         const uint32_t now_marks = marks, now_live = live;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
           now_pairs[i] = pairs[i];
-#pragma unroll
-          for (int n = 0; n < kLoads; ++n) now[i][n] = codes[i][n];
+          now[i] = codes[i];
         }
         if (step + 1 < steps) load(step + 1);
         if (j >= kStages) fine = warp_wait(&empty[stage], (j / kStages - 1) & 1, &abort_flag);
         if (!fine) break;
-        if (now_live != (1u << kPasses) - 1) {
+        if (now_live != (1u << kRunsOfTile) - 1 || (begin + j + 1) * kKeys > keys) {
 #pragma unroll
           for (int i = 0; i < kPasses; ++i) {
-            if (now_live >> i & 1) continue;
+            const int row = kPassRows * i + lane_row;
+            if ((now_live >> (row / 16) & 1) && (begin + j) * kKeys + row < keys) continue;
             now_pairs[i] = 0;
-#pragma unroll
-            for (int n = 0; n < kLoads; ++n) now[i][n] = make_uint4(0, 0, 0, 0);
+            now[i] = make_uint4(0, 0, 0, 0);
           }
         }
         uint8_t* const tile = (side ? v_smem : k_smem) + stage * Cfg::kTileBytes;
@@ -546,24 +582,28 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           const int row = kPassRows * i + lane_row;
           const float zero = 128.f + bf16_hi(now_pairs[i]);
           const uint32_t zeros = pack2(zero, zero);
-          if (lane_piece == 0) {
-            (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]);
-          }
+          if (lane_piece == 0) (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]);
+          uint32_t words[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
 #pragma unroll
-          for (int n = 0; n < kLoads; ++n) {
-            const int piece = lane_piece + 4 * n;
-            const uint32_t words[4] = {now[i][n].x, now[i][n].y, now[i][n].z, now[i][n].w};
-            uint8_t* const segment = tile + (piece / 2) * (kKeys * 128) + row * 128;
+          for (int bit = 1; kDim == 256 && bit < 4; bit *= 2)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              uint32_t v[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[e] = ((words[w] >> (4 * e)) & 0x000f000fu) | 0x43004300u;
-                asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v[e]) : "r"(zeros));
-              }
-              *reinterpret_cast<uint4*>(segment + (((piece % 2) * 4 + w) ^ (row & 7)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+              if (w & bit) continue;
+              const uint32_t first = words[w], second = words[w ^ bit];
+              words[w] = turn & bit ? second : first;
+              words[w ^ bit] = turn & bit ? first : second;
             }
+          uint8_t* const segment = tile + (lane_piece / 2) * (kKeys * 128) + row * 128;
+          const int chunk = (lane_piece % 2 * 4) ^ turn ^ (row & 7);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[e] = ((words[w] >> (4 * e)) & 0x000f000fu) | 0x43004300u;
+              asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v[e]) : "r"(zeros));
+            }
+            *reinterpret_cast<uint4*>(segment + (chunk ^ w) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         if (side == 0) {
@@ -575,11 +615,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           if (now_marks) {
             any_hidden[j % kKv4MarkSlots] = 1;
             atomicOr(&g_ci8_status, kStatusBadIndex);
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-              const int row = kPassRows * i + lane_row;
-              if (now_marks >> i & 1) atomicOr(&hidden[j % kKv4MarkSlots][row / 32], 1u << (row % 32));
-            }
+            if (now_marks >> lane & 1) atomicOr(&hidden[j % kKv4MarkSlots][lane / 2], 0xffffu << (lane % 2 * 16));
           }
           mbar_arrive(smem_u32(&bar_scale_k[slot]));
         } else {
@@ -597,12 +633,18 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         const uint32_t v_desc = desc_low(smem_u32(v_smem), kKeys * 128);
         constexpr uint32_t kTileStep = Cfg::kTileBytes / 16, kQStep = Cfg::kQBytes / 16;
         auto scores = [&](int t, int buffer, int stage) {
-          const uint32_t d = tmem + 128 * buffer, a = q_desc + t * kQStep, b = k_desc + stage * kTileStep;
+          const uint32_t d = tmem + Cfg::kScoreColumns * buffer, b = k_desc + stage * kTileStep;
+          const uint32_t a = Cfg::kQInTmem ? tmem + Cfg::kQColumn + t * (kDim / 2) : q_desc + t * kQStep;
           if (elect_one()) {
 #pragma unroll
             for (int s = 0; s < kSegments; ++s)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) mma_bf16_ss(d, a + s * (128 * 128 / 16) + 2 * k, b + s * (kKeys * 128 / 16) + 2 * k, kIdescS, s + k > 0);
+              for (int k = 0; k < 4; ++k) {
+                if constexpr (Cfg::kQInTmem)
+                  mma_bf16_ts(d, a + 32 * s + 8 * k, b + s * (kKeys * 128 / 16) + 2 * k, kIdescS, s + k > 0);
+                else
+                  mma_bf16_ss(d, a + s * (128 * 128 / 16) + 2 * k, b + s * (kKeys * 128 / 16) + 2 * k, kIdescS, s + k > 0);
+              }
             mma_commit(smem_u32(&bar_s[buffer]));
           }
           __syncwarp();
@@ -611,7 +653,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           for (int h = 0; h < kKeys / 64; ++h) {
             if (!warp_wait(&bar_p[buffer][h], parity, &abort_flag)) return false;
             tcgen05_fence_after();
-            const uint32_t d = tmem + kOutputColumn + t * kDim, a = tmem + 128 * buffer + 32 * h, b = v_desc + stage * kTileStep + h * (8192 / 16);
+            const uint32_t d = tmem + kOutputColumn + t * kDim, a = tmem + Cfg::kScoreColumns * buffer + 32 * h, b = v_desc + stage * kTileStep + h * (8192 / 16);
             if (elect_one()) {
               mma_bf16_ts(d, a, b, kIdescO, accumulate || h > 0);
 #pragma unroll
@@ -706,12 +748,12 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const Kv4PromptPar
     auto piece = [&](int s) { return base + (static_cast<int64_t>(s) * Cfg::kRows + row / 128 * 128) * (kDim + 2); };
     float most = -INFINITY, all = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < params.splits; ++s) most = fmaxf(most, piece(s)[row % 128]);
+    for (int s = 0; s < params.splits; ++s) most = fmaxf(most, __ldcg(piece(s) + row % 128));
     for (int s = 0; s < params.splits; ++s) {
-      const float sum = piece(s)[128 + row % 128];
+      const float sum = __ldcg(piece(s) + 128 + row % 128);
       if (sum == 0.f) continue;                          // saw no key (a NaN score makes its sum NaN, which is kept)
-      const float weight = kv4_exp2(piece(s)[row % 128] - most);
-      const float4 y = *reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column);
+      const float weight = kv4_exp2(__ldcg(piece(s) + row % 128) - most);
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column));
       all += weight * sum;
       x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
     }
