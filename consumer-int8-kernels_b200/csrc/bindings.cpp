@@ -578,8 +578,8 @@ void boxed_kv4_attention(StableIValue* stack, uint64_t, uint64_t) {
   check(kv_lens, ScalarType::Int, device);
   check(workspace, ScalarType::Byte, device);
   STD_TORCH_CHECK(kv_lens.dim() == 1 && block_table.dim() == 2 && block_table.size(0) == kv_lens.size(0) && q_starts.dim() == 1 &&
-                      q_starts.size(0) == kv_lens.size(0) + 1 && block_table.numel() <= kIntMax && block_table.size(1) * c.page <= kIntMax,
-                  "Expected INT32 block_table [batch, width], q_starts [batch + 1] and kv_lens [batch]");
+                      q_starts.size(0) == kv_lens.size(0) + 1 && block_table.numel() <= kIntMax && block_table.size(1) * c.page <= (1ll << 30),
+                  "Expected INT32 block_table [batch, width] (pages of 2^30 tokens at most), q_starts [batch + 1] and kv_lens [batch]");
   STD_TORCH_CHECK(workspace.numel() >= ci8_kv4_workspace_bytes() && address(workspace) % 16 == 0,
                   "The attention workspace is too small or not aligned");
   STD_TORCH_CHECK(scale > 0 && scale < 3.0e38, "The softmax scale must be positive and finite");

@@ -1410,7 +1410,7 @@ int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, cons
   if (tokens == 0 || batch == 0) return 0;
   if (!kv4_row_source(q, q_stride, tokens, q_heads, dim) || (pages > 0 && !cache) || !aligned(cache, 16) || (width > 0 && !block_table) ||
       !aligned(block_table, 4) || !q_starts || !aligned(q_starts, 4) || !kv_lens || !aligned(kv_lens, 4) || !workspace ||
-      !aligned(workspace, 16) || !out || !aligned(out, 16) || (static_cast<long long>(width) << shift) > 0x7fffffffll)
+      !aligned(workspace, 16) || !out || !aligned(out, 16) || (static_cast<long long>(width) << shift) > (1ll << 30))
     return kInvalid;
   Kv4AttendParams p = {};
   p.q = static_cast<const uint16_t*>(q); p.q_stride = q_stride; p.cache = static_cast<const uint8_t*>(cache);
