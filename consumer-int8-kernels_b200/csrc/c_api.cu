@@ -842,6 +842,8 @@ bool kv4_rotation(const float* cos_sin, int table_rows, int rotary, const int64_
 
 // How many warps share the heads of one token, `steps` loads each at most: enough warps to fill the GPU a few times over
 // where the tokens are few (a generated token: 28 heads of 256 components on 28 warps), whole batches of loads otherwise.
+// Norm, us on the device, one warp a token, this rule, one load a warp: 1 token 7.4, 2.2, 2.2; 300 tokens of 32 and 8 heads
+// of 128 6.3, 4.6, 4.6; 16384 tokens 69, 68, 167.
 int kv4_chunks(int tokens, long long steps, long long batch) {
   const long long busy = static_cast<long long>(sm_count()) * 128;
   long long chunks = (busy + tokens - 1) / tokens;
@@ -912,7 +914,8 @@ int launch_kv4_single(const Kv4AttendParams& a, void* workspace, int most_rows, 
                                      : launch_kv4_single_q<kDim, 2>(a, workspace, most_rows, stream);
 }
 
-// Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys and a second kernel joins.
+// Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys and a second kernel joins (us,
+// unsplit and split: 64 tokens over 8192 keys, 32 and 8 heads of 128, 205 and 65; 256 tokens, 24 and 4 heads of 256, 184 and 112).
 template <int kDim>
 int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
   using Cfg = Kv4PromptConfig<kDim>;
@@ -940,10 +943,13 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
   if (code || p.splits == 1) return code;
   return launch_pdl(kv4_prompt_join_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, 8), 256, 0, stream, p);
 }
-// Sequences with few rows go to the kernel for generated tokens, the others to the one for prompts; which they are is
-// only known on the device, so each kernel passes over the other's. No sequence has more than one row (or the rows
-// happen to be spread unevenly) when there are no more rows than sequences: one kernel.
-constexpr int kKv4FewRows = 16;
+// Sequences with few query rows (tokens times heads per key head) go to the kernel for generated tokens, the others to the
+// one for prompts; which they are is only known on the device, so each kernel passes over the other's. The one takes time
+// with every eight rows, the other with every 128 or 256. Measured (us, the one and the other): 64 sequences of 4096 keys,
+// 8 key heads of 128, 32 rows 230 and 548, 64 rows 470 and 550, 128 rows 660 and 483; 16 sequences, 4 heads of 256, 48 rows
+// 102 and 118, 120 rows 245 and 117; one sequence of 8192 keys, 64 rows 30 and 42, 128 rows 42 and 48. No sequence has more
+// than one row (or the rows happen to be spread unevenly) when there are no more rows than sequences: one kernel.
+constexpr int kKv4FewRows = 64;
 template <int kDim>
 int launch_kv4_attention(const Kv4AttendParams& a, void* workspace, ci8_stream_t stream) {
   if (a.tokens <= a.batch) return launch_kv4_single<kDim>(a, workspace, 0x7fffffff, stream);

@@ -128,6 +128,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // rotation needs no exchange between lanes; otherwise its runs are neighbours. FP32 throughout, two components to an
 // instruction where nothing speaks against it. Bound by memory: 4 bytes per component of the norm, 2 read and
 // dim / 2 + 4 bytes per head written for what is appended.
+// Measured: norm of 16384 tokens, 32 and 8 heads of 128, 68 us (5.1 TB/s of a measured copy's 6.5); of 4099 tokens, 16 and
+// 16 heads of 64, 8.3 us on the device; of one token 2.2 us; appending 8192 tokens, 32 and 8 heads of 128, and reading them
+// back 62 us (3.7 TB/s). One warp for all heads of a token, keys and queries mixed, took 112 and 100 us.
 template <int kDim, bool kNorm, bool kAppend, bool kAdjacent>
 __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) {
   constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 4;
@@ -326,7 +329,8 @@ struct Kv4ReadParams {
 
 // One warp takes a piece of one token's heads (keys', then values'): eight codes (one word) per lane become eight BF16
 // values. Two codes behind a mask are the BF16 numbers 128 + code; the zero point comes off exactly and the product
-// with the scale is rounded once. Bound by memory (dim / 2 + 4 bytes read, 2 dim written per head).
+// with the scale is rounded once. Bound by memory (dim / 2 + 4 bytes read, 2 dim written per head). Measured: 65536 tokens,
+// 8 heads of 128, 62 us (5.5 TB/s); one CTA per token and head took 126.
 template <int kDim>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4ReadParams p) {
   constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 8;

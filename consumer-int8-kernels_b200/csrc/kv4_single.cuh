@@ -1,8 +1,12 @@
 // Attention of few query rows per sequence (generated tokens) over the 4-bit key/value cache: bound by reading the
-// cache, dim / 2 + 4 bytes per token and side.
+// cache, dim / 2 + 4 bytes per token and side, and as much by the instructions that unpack it: 530 for a warp's 32 keys of 128
+// components (16 + 16 of them matrix products), with the schedulers issuing in 56 % of the cycles and the logic pipe
+// busy in 50 %. Measured: 64 sequences of up to 8192 keys, 32 query heads and 8 key heads of 128, 75 us (4.0 TB/s); 4 of 65536,
+// 24 and 4 heads of 256, 78 us (3.6 TB/s); one of 1000 keys 11.5 us, most of it a chain of dependent loads and joins. The same
+// loads without the arithmetic reach 5.6 TB/s.
 //
-// Work is cut into tiles of 32 tokens of one (sequence, key head, block of query rows) and the tiles of all of them,
-// laid end to end, are dealt to the warps in equal contiguous ranges, so that ragged batches fill the GPU evenly and
+// Work is cut into tiles of 64 tokens (32 for dim 256) of one (sequence, key head, block of query rows) and the tiles of all of
+// them, laid end to end, are dealt to the warps in equal contiguous ranges, so that ragged batches fill the GPU evenly and
 // a long history is split as far as there are warps. Every warp runs on its own: its ring of tiles is filled by
 // asynchronous copies it issues itself, and it keeps its own running maximum, sum and output. Ranges begin and end inside a
 // sequence; what a warp has of such a sequence is joined with its neighbours' inside the CTA at the end, and across
@@ -243,7 +247,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     return;
   }
   const unsigned total = static_cast<unsigned>(all_tiles);
-  // No more CTAs than get kLeast tiles each: below that, joining them costs more than the tiles.
+  // No more CTAs than get kLeast tiles each: below that, joining them costs more than the tiles. Measured (us for 1, 4, 16):
+  // one sequence of 100 keys, 8 key heads of 128, 10.4, 7.7, 11.8; of 1000 12.2, 11.5, 13.5; of 8000 15.1, 15.4, 20.3.
   constexpr unsigned kLeast = 4;
   const unsigned ctas = min(gridDim.x, (total + kLeast - 1) / kLeast);
   if (blockIdx.x >= ctas) return;
@@ -535,48 +540,46 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         int high[2][kQ][4], low[2][kQ][4];
 #pragma unroll
         for (int j = 0; j < kKWords; j += kLoad) {
-          uint32_t wa[2][kLoad], wb[2][kLoad];
+          uint32_t wa[2][kLoad], wb[2][kLoad];           // two parts side by side: four independent sums
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-          const uint8_t* at = keys_at + 16 * (m2 + u) * (kDim / 2) + (key_at ^ 16 * j);
-          lds_words(at, wa[u]);
-          lds_words(at + 8 * (kDim / 2), wb[u]);
+            const uint8_t* at = keys_at + 16 * (m2 + u) * (kDim / 2) + (key_at ^ 16 * j);
+            lds_words(at, wa[u]);
+            lds_words(at + 8 * (kDim / 2), wb[u]);
           }
 #pragma unroll
-          for (int k = 0; k < kLoad; ++k) {
+          for (int k = 0; k < kLoad; ++k)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t a0 = wa[u][k] & 0x0f0f0f0fu, a1 = wb[u][k] & 0x0f0f0f0fu, a2 = (wa[u][k] >> 4) & 0x0f0f0f0fu, a3 = (wb[u][k] >> 4) & 0x0f0f0f0fu;
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a0 = wa[u][k] & 0x0f0f0f0fu, a1 = wb[u][k] & 0x0f0f0f0fu, a2 = (wa[u][k] >> 4) & 0x0f0f0f0fu, a3 = (wb[u][k] >> 4) & 0x0f0f0f0fu;
 #pragma unroll
-            for (int n = 0; n < kQ; ++n) {
-              const uint32_t(&d)[4] = q[j + k][n];
-              if (j + k == 0) {
-                mma_u8s8_first(high[u][n], a0, a1, a2, a3, d[0], d[1]);
-                mma_u8s8_first(low[u][n], a0, a1, a2, a3, d[2], d[3]);
-              } else {
-                mma_u8s8(high[u][n], a0, a1, a2, a3, d[0], d[1]);
-                mma_u8s8(low[u][n], a0, a1, a2, a3, d[2], d[3]);
+              for (int n = 0; n < kQ; ++n) {
+                const uint32_t(&d)[4] = q[j + k][n];
+                if (j + k == 0) {
+                  mma_u8s8_first(high[u][n], a0, a1, a2, a3, d[0], d[1]);
+                  mma_u8s8_first(low[u][n], a0, a1, a2, a3, d[2], d[3]);
+                } else {
+                  mma_u8s8(high[u][n], a0, a1, a2, a3, d[0], d[1]);
+                  mma_u8s8(low[u][n], a0, a1, a2, a3, d[2], d[3]);
+                }
               }
             }
-          }
-          }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int mt = m2 + u;
-          const int t = 16 * mt + turned + 8 * r;
-          const uint32_t key_pair = lds32(keys_at + Cfg::kCodeBytes + 4 * t);
-          vscale[mt][r] = bf16_lo(lds32(values_at + Cfg::kCodeBytes + 4 * t));
-          const float kscale = bf16_lo(key_pair);
-          const int zero = __float2int_rn(bf16_hi(key_pair));
+          for (int r = 0; r < 2; ++r) {
+            const int mt = m2 + u, t = 16 * mt + turned + 8 * r;
+            const uint32_t key_pair = lds32(keys_at + Cfg::kCodeBytes + 4 * t);
+            vscale[mt][r] = bf16_lo(lds32(values_at + Cfg::kCodeBytes + 4 * t));
+            const float kscale = bf16_lo(key_pair);
+            const int zero = __float2int_rn(bf16_hi(key_pair));
 #pragma unroll
-          for (int n = 0; n < kQ; ++n)
+            for (int n = 0; n < kQ; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              s[mt][n][2 * r + e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]) * kscale;
-        }
+              for (int e = 0; e < 2; ++e)
+                s[mt][n][2 * r + e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]) * kscale;
+          }
       }
       if (!whole) {
 #pragma unroll

@@ -129,3 +129,24 @@ def test_tables_of_more_than_2_to_the_30_tokens_are_refused(ops, workspace):
     table = torch.zeros(1, 2 ** 26 + 1, dtype=torch.int32, device=DEV)
     with pytest.raises(RuntimeError, match="block_table"):
         ops.kv4_attention(q, cache, table, starts, lens, workspace, torch.empty_like(q), case.scale)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (2, 2), (14, 2)])
+def test_rows_on_either_side_of_the_kernels_border(ops, workspace, dim, q_heads, kv_heads):
+    """Sequences of one query row, of a few blocks of rows and of one row more than those, in one call."""
+    group = q_heads // kv_heads
+    around = [max(1, 64 // group + d) for d in (-1, 0, 1, 2)]
+    run_and_check(ops, workspace, Case([(n, n + 75) for n in around] + [(1, 30), (n := 130 // group + 1, n)], q_heads, kv_heads, dim, 16, seed=dim + group))
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (256, 16), (64, 256), (128, 64), (256, 128)])
+def test_bad_pages_among_a_prompts_keys(ops, workspace, dim, page):
+    """Page numbers outside the cache at a tile's start, middle and end, and in a sequence's last, partly filled page."""
+    case = Case([(90, 3 * 256 + 5), (130, 700), (100, 100)], 4, 2, dim, page, seed=page + dim)
+    pages = case.cache.shape[0]
+    case.table[0, 0] = pages
+    case.table[0, -(-(3 * 256 + 5) // page) - 1] = -7
+    case.table[1, 700 // page // 2] = 2 ** 31 - 1
+    case.table[1, (700 // page // 2) + 1] = -1
+    run_and_check(ops, workspace, case, status=8)
