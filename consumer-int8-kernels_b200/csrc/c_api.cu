@@ -915,12 +915,16 @@ int launch_kv4_single(const Kv4AttendParams& a, void* workspace, int most_rows, 
 }
 
 // Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys and a second kernel joins (us,
-// unsplit and split: 64 tokens over 8192 keys, 32 and 8 heads of 128, 205 and 65; 256 tokens, 24 and 4 heads of 256, 184 and 112).
+// unsplit and split: 64 tokens over 8192 keys, 32 and 8 heads of 128, 205 and 65; 256 tokens, 24 and 4 heads of 256, 184 and
+// 112; 2 ragged sequences of up to 13 tokens over up to 27071 keys, 7 heads of 64 on one, 16 parts 71, as many as fit 54). Where
+// they fill more than half of it, a few parts each even the load out, if they are long: 3 sequences of 1093 tokens over 6718
+// keys, 7 heads of 64 on one, 179 and 133; but 426 tokens over 872 keys, 16 and 8 heads of 256, 34 and 62 with 4 tiles a part.
 template <int kDim>
 int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
   using Cfg = Kv4PromptConfig<kDim>;
-  static std::atomic<uint64_t> raised{0};
-  const cudaError_t err = ensure_smem(kv4_prompt_kernel<kDim>, Cfg::kSmemBytes, raised);
+  static std::atomic<uint64_t> raised{0}, raised_split{0};
+  cudaError_t err = ensure_smem(kv4_prompt_kernel<kDim, false>, Cfg::kSmemBytes, raised);
+  if (err == cudaSuccess) err = ensure_smem(kv4_prompt_kernel<kDim, true>, Cfg::kSmemBytes, raised_split);
   if (err != cudaSuccess) return static_cast<int>(err);
   const long long all_rows = static_cast<long long>(a.tokens) * a.group.d;
   long long sequences = all_rows / (most_rows + 1);       // that have more rows than most_rows
@@ -929,9 +933,10 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
   if (tiles == 0) return 0;
   if (tiles > 0x7fffffffll) return kInvalid;
   const long long key_tiles = ((static_cast<long long>(a.width) << a.page_shift) + Cfg::kKeys - 1) / Cfg::kKeys;
-  long long splits = sm_count() / (tiles * a.kv_heads);
-  if (splits > key_tiles / 4) splits = key_tiles / 4;
-  if (splits > 16) splits = 16;
+  const long long jobs = tiles * a.kv_heads, sms = sm_count();
+  long long splits = 2 * jobs <= sms ? sms / jobs : jobs < sms ? 4 : 1;
+  const long long least = 2 * jobs <= sms ? 4 : 16;      // tiles of keys in a part
+  if (splits > key_tiles / least) splits = key_tiles / least;
   const long long slot = static_cast<long long>(Cfg::kRows) * (kDim + 2) * 4;
   while (splits > 1 && kKv4CounterBytes + tiles * a.kv_heads * splits * slot > kKv4WorkspaceBytes) --splits;
   Kv4PromptParams p;
@@ -939,7 +944,7 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
   p.splits = splits > 1 ? static_cast<int>(splits) : 1;
   p.partial = splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kKv4CounterBytes) : nullptr;
   p.most_rows = most_rows;
-  const int code = launch_pdl(kv4_prompt_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, p.splits), Cfg::kThreads, Cfg::kSmemBytes, stream, p);
+  const int code = launch_pdl(p.splits > 1 ? kv4_prompt_kernel<kDim, true> : kv4_prompt_kernel<kDim, false>, dim3(static_cast<unsigned>(tiles), a.kv_heads, p.splits), Cfg::kThreads, Cfg::kSmemBytes, stream, p);
   if (code || p.splits == 1) return code;
   return launch_pdl(kv4_prompt_join_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, 8), 256, 0, stream, p);
 }

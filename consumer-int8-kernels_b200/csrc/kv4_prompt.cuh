@@ -14,8 +14,8 @@
 // What bounds it is not the tensor pipe (a third busy) but what feeds it. Dim 256, where a tile of keys serves 128 rows
 // only: the unpacking (11 instructions and one 16-byte store for eight components), ahead of the shared memory's bandwidth.
 // Dim 128: the chain scores -> softmax -> product -> next scores of each query tile, of which two run at a time, with 39 %
-// of the cycles taken by the exponentials. Measured (32 query heads and 8 key heads of 128, 8192 new tokens): 775 us,
-// 710 TFLOP/s; 24 and 4 heads of 256, 4096 tokens behind 4096: 779 us, 794 TFLOP/s, where queries in shared memory and lanes
+// of the cycles taken by the exponentials. Measured (32 query heads and 8 key heads of 128, 8192 new tokens): 747 us,
+// 736 TFLOP/s; 24 and 4 heads of 256, 4096 tokens behind 4096: 779 us, 794 TFLOP/s, where queries in shared memory and lanes
 // that load from eight rows at a time took 1020; 32 and 8 heads of 64, 8192 tokens: 629 us. Tried and slower: tiles of 64 keys
 // with two score buffers for dim 128 (792), the tiles of keys dealt to two softmax warpgroups in turn (831; dim 256 880
 // against 876 then), four unpacking warpgroups for dim 256 (917 against 876), more registers for the softmax (782 to 821).
@@ -50,7 +50,7 @@ struct Kv4PromptConfig {
 
 struct Kv4PromptParams {
   Kv4AttendParams a;
-  float* partial;             // [tile][key head][split][maximum, sum, output of every row], null: one split
+  float* partial;             // [tile][key head][split][maximum, sum, output of every row] where there are several splits
   int splits;
   int most_rows;              // sequences with no more query rows than this belong to another kernel
 };
@@ -169,7 +169,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, int parity, int* abort)
   return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort));
 }
 
-template <int kDim>
+// kSplit: a row tile's keys are split over gridDim.z CTAs, whose parts the kernel below joins. (In one kernel for both, the
+// loops' values got worse registers: 8192 tokens of 32 and 8 heads of 128 took 775 us, 747 in the one without splits.)
+template <int kDim, bool kSplit>
 __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParams params) {
   using Cfg = Kv4PromptConfig<kDim>;
   constexpr int kQTiles = Cfg::kQTiles, kKeys = Cfg::kKeys, kStages = Cfg::kStages;
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = tmem_base;
-  const int b = tile_info[0], first_row = tile_info[1] * Cfg::kRows, head = blockIdx.y, split = blockIdx.z;
+  const int b = tile_info[0], first_row = tile_info[1] * Cfg::kRows, head = blockIdx.y, split = kSplit ? blockIdx.z : 0;
   const int group = p.group.d;
 
   if (b >= 0) {
@@ -249,8 +251,8 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
     const int last_row = min(all_rows, first_row + Cfg::kRows) - 1;
     const int keys = max(0, seq.keys - seq.rows + p.group.quotient(last_row) + 1);   // that the CTA's last row sees
     const int all_tiles = (keys + kKeys - 1) / kKeys;
-    const int begin = static_cast<int>(static_cast<long long>(all_tiles) * split / params.splits);
-    const int end = static_cast<int>(static_cast<long long>(all_tiles) * (split + 1) / params.splits);
+    const int begin = kSplit ? static_cast<int>(static_cast<long long>(all_tiles) * split / params.splits) : 0;
+    const int end = kSplit ? static_cast<int>(static_cast<long long>(all_tiles) * (split + 1) / params.splits) : all_tiles;
     const int tiles = end - begin;
 
     if (warpgroup < kSoftmaxGroups) {
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
       // ---- output
       if (fine && tiles > 0) fine = warp_wait(&bar_done[t], 0, &abort_flag);
       tcgen05_fence_after();
-      if (params.partial) {
+      if constexpr (kSplit) {
         float* slot = params.partial + (((static_cast<int64_t>(blockIdx.x) * p.kv_heads + head) * params.splits + split) * Cfg::kRows + 128 * t) * (kDim + 2);
         slot[row_in_tile] = row_max[t][row_in_tile];       // [128 maxima][128 sums][128 outputs]
         slot[128 + row_in_tile] = sum;
