@@ -914,11 +914,12 @@ int launch_kv4_single(const Kv4AttendParams& a, void* workspace, int most_rows, 
                                      : launch_kv4_single_q<kDim, 2>(a, workspace, most_rows, stream);
 }
 
-// Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys and a second kernel joins (us,
-// unsplit and split: 64 tokens over 8192 keys, 32 and 8 heads of 128, 205 and 65; 256 tokens, 24 and 4 heads of 256, 184 and
-// 112; 2 ragged sequences of up to 13 tokens over up to 27071 keys, 7 heads of 64 on one, 16 parts 71, as many as fit 54). Where
-// they fill more than half of it, a few parts each even the load out, if they are long: 3 sequences of 1093 tokens over 6718
-// keys, 7 heads of 64 on one, 179 and 133; but 426 tokens over 872 keys, 16 and 8 heads of 256, 34 and 62 with 4 tiles a part.
+// Prompts. Where the row tiles are too few to fill the GPU, each is split along the keys, in parts of four tiles of keys at
+// least, and a second kernel joins (us, unsplit and split: 64 tokens over 8192 keys, 32 and 8 heads of 128, 205 and 65; 256
+// tokens, 24 and 4 heads of 256, 184 and 112; up to 16 parts and as many as fit: 2 sequences of up to 13 tokens over up to 27071
+// keys, 7 heads of 64 on one, 71 and 51). Several sequences are of different lengths: three waves of parts, if these have 16
+// tiles, even that out (one wave and three: 6 sequences of up to 163 tokens over up to 11938 keys, 8 and 8 heads of 256, 231 and
+// 181; 7 of up to 126 over up to 28862 240 and 191; but one of 704 tokens over 18522 keys, 8 and 2 heads of 64, 82 and 109).
 template <int kDim>
 int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, ci8_stream_t stream) {
   using Cfg = Kv4PromptConfig<kDim>;
@@ -934,9 +935,10 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
   if (tiles > 0x7fffffffll) return kInvalid;
   const long long key_tiles = ((static_cast<long long>(a.width) << a.page_shift) + Cfg::kKeys - 1) / Cfg::kKeys;
   const long long jobs = tiles * a.kv_heads, sms = sm_count();
-  long long splits = 2 * jobs <= sms ? sms / jobs : jobs < sms ? 4 : 1;
-  const long long least = 2 * jobs <= sms ? 4 : 16;      // tiles of keys in a part
-  if (splits > key_tiles / least) splits = key_tiles / least;
+  long long splits = sms / jobs, even = (a.batch > 2 ? 3 : 1) * sms / jobs;
+  if (splits > key_tiles / 4) splits = key_tiles / 4;
+  if (even > key_tiles / 16) even = key_tiles / 16;
+  if (splits < even) splits = even;
   const long long slot = static_cast<long long>(Cfg::kRows) * (kDim + 2) * 4;
   while (splits > 1 && kKv4CounterBytes + tiles * a.kv_heads * splits * slot > kKv4WorkspaceBytes) --splits;
   Kv4PromptParams p;
@@ -946,7 +948,10 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
   p.most_rows = most_rows;
   const int code = launch_pdl(p.splits > 1 ? kv4_prompt_kernel<kDim, true> : kv4_prompt_kernel<kDim, false>, dim3(static_cast<unsigned>(tiles), a.kv_heads, p.splits), Cfg::kThreads, Cfg::kSmemBytes, stream, p);
   if (code || p.splits == 1) return code;
-  return launch_pdl(kv4_prompt_join_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, 8), 256, 0, stream, p);
+  // about two waves of the join's CTAs, a thread no more than one group of four components where that is enough
+  long long share = 16 * sms / jobs;
+  if (share > Cfg::kRows * kDim / 4 / 256) share = Cfg::kRows * kDim / 4 / 256;
+  return launch_pdl(kv4_prompt_join_kernel<kDim>, dim3(static_cast<unsigned>(tiles), a.kv_heads, static_cast<unsigned>(share)), 256, 0, stream, p);
 }
 // Sequences with few query rows (tokens times heads per key head) go to the kernel for generated tokens, the others to the
 // one for prompts; which they are is only known on the device, so each kernel passes over the other's. The one takes time

@@ -750,12 +750,15 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const Kv4PromptPar
     auto piece = [&](int s) { return base + (static_cast<int64_t>(s) * Cfg::kRows + row / 128 * 128) * (kDim + 2); };
     float most = -INFINITY, all = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
     for (int s = 0; s < params.splits; ++s) most = fmaxf(most, __ldcg(piece(s) + row % 128));
+#pragma unroll 4
     for (int s = 0; s < params.splits; ++s) {
-      const float sum = __ldcg(piece(s) + 128 + row % 128);
-      if (sum == 0.f) continue;                          // saw no key (a NaN score makes its sum NaN, which is kept)
-      const float weight = kv4_exp2(__ldcg(piece(s) + row % 128) - most);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column));
+      const float sum = __ldcg(piece(s) + 128 + row % 128), top = __ldcg(piece(s) + row % 128);
+      float4 y = __ldcg(reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column));
+      // a part that saw no key has sum 0 and left its output unwritten (a NaN score makes its sum NaN, which is kept)
+      const float weight = sum == 0.f ? 0.f : kv4_exp2(top - most);
+      if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
       all += weight * sum;
       x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
     }
