@@ -129,8 +129,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // instruction where nothing speaks against it. Bound by memory: 4 bytes per component of the norm, 2 read and
 // dim / 2 + 4 bytes per head written for what is appended.
 // Measured: norm of 16384 tokens, 32 and 8 heads of 128, 68 us (5.1 TB/s of a measured copy's 6.5); of 4099 tokens, 16 and
-// 16 heads of 64, 8.3 us on the device; of one token 2.2 us; appending 8192 tokens, 32 and 8 heads of 128, and reading them
-// back 62 us (3.7 TB/s). One warp for all heads of a token, keys and queries mixed, took 112 and 100 us.
+// 16 heads of 64, 8.3 us on the device; of one token 2.2 us; appending 8192 tokens, 32 and 8 heads of 128, 51 us: the queries
+// 26 (5.1 TB/s), keys and values 24, bound by instruction issue (67 % of the cycles; 20 without the repairs of ties, which
+// BF16 inputs meet in most warps' steps). One warp for all heads of a token, keys and queries mixed, took 112 for that norm.
+// 64 registers and four CTAs of 256 threads an SM: three 52, five 118 us for that append (spills).
 template <int kDim, bool kNorm, bool kAppend, bool kAdjacent>
 __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) {
   constexpr int kLanes = kDim / 8, kHeadsPerStep = 32 / kLanes, kBatch = 4;
