@@ -150,3 +150,31 @@ def test_bad_pages_among_a_prompts_keys(ops, workspace, dim, page):
     case.table[1, 700 // page // 2] = 2 ** 31 - 1
     case.table[1, (700 // page // 2) + 1] = -1
     run_and_check(ops, workspace, case, status=8)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,sequences", [
+    (128, 96, 1, [(1, 70), (1, 333)]), (128, 96, 1, [(1, 70), (3, 150), (0, 9)]), (64, 1024, 1, [(1, 40), (1, 5)]),
+    (64, 1024, 1, [(2, 90)]), (256, 260, 260, [(1, 20), (1, 33)]), (64, 130, 130, [(70, 90), (1, 33)])])
+def test_many_heads(ops, workspace, dim, q_heads, kv_heads, sequences):
+    """More query heads on a key head than a tile has rows, and more key heads than there are multiprocessors."""
+    run_and_check(ops, workspace, Case(sequences, q_heads, kv_heads, dim, 16, seed=q_heads + len(sequences)))
+
+
+def test_many_heads_in_the_row_operators(ops):
+    """1024 query heads and 1024 key heads: appended, read back and compared with the checker; the norm against its definition."""
+    dim, page, tokens, heads = 64, 16, 3, 1024
+    g = torch.Generator().manual_seed(101)
+    q, k, v = (torch.randn(tokens, heads, dim, generator=g).bfloat16() for _ in range(3))
+    cache = torch.zeros(1, 2, heads, ref.block_bytes(page, dim), dtype=torch.uint8)
+    on_device = cache.to(DEV)
+    slots = torch.tensor([15, 0, 7])
+    ops.kv4_append(None, k.to(DEV), v.to(DEV), None, None, None, slots.to(DEV), None, on_device)
+    ref.store(cache, slots, k.float(), v.float())
+    assert_bit_equal(on_device, cache.to(DEV), "cache")
+    weight = torch.rand(dim, generator=g).bfloat16()
+    q_out, k_out = torch.empty_like(q, device=DEV), torch.empty_like(k, device=DEV)
+    ops.qk_norm_rope(q.to(DEV), k.to(DEV), weight.to(DEV), weight.to(DEV), None, None, None, q_out, k_out)
+    for got, x in ((q_out, q), (k_out, k)):
+        want = x.double() * (x.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt() * weight.double()
+        # one rounding to BF16; FP32 before it: 64 squares and their sum, rsqrt within 2 units, three products: 2^-20 in all
+        assert bool(((got.cpu().double() - want).abs() <= (2.0 ** -8 + 2.0 ** -20) * want.abs()).all())
