@@ -29,11 +29,13 @@ class Kv4AttentionLayer:
     ``w_qkv`` INT8 [(q_heads + 2 kv_heads) * dim, K] with BF16 channel scales, ``w_out`` INT8 [N, q_heads * dim] likewise;
     ``q_weight`` / ``k_weight`` BF16 [dim] norm weights or None (no norm), ``cos_sin`` FP32 [rows, rotary] or None (no
     rotation). Without norm weights the rotation of queries and keys is part of the append and one launch is saved.
+    ``workspace`` (UINT8 [``kv4_workspace_bytes()``], zeroed once) may be shared by layers that run one after the other; by
+    default the layer has its own.
     """
 
     def __init__(self, w_qkv, qkv_scale, w_out, out_scale, q_heads: int, kv_heads: int, dim: int, max_tokens: int,
                  q_weight=None, k_weight=None, cos_sin=None, eps: float = 1e-6, weight_offset: float = 0.0,
-                 adjacent: bool = False, scale: float | None = None, operators=None):
+                 adjacent: bool = False, scale: float | None = None, workspace=None, operators=None):
         if operators is None:
             from . import ops as operators  # the compiled operators; there is no fallback
 
@@ -62,7 +64,11 @@ class Kv4AttentionLayer:
         self.attended = torch.empty(max_tokens, q_heads, dim, **bf16)
         self.attended_codes = torch.empty(max_tokens, q_heads * dim, dtype=torch.int8, device=device)
         self.out = torch.empty(max_tokens, w_out.shape[0], **bf16)
-        self.workspace = torch.zeros(operators.kv4_workspace_bytes(), dtype=torch.uint8, device=device)
+        if workspace is None:
+            workspace = torch.zeros(operators.kv4_workspace_bytes(), dtype=torch.uint8, device=device)
+        elif workspace.dtype != torch.uint8 or workspace.device != device or workspace.numel() < operators.kv4_workspace_bytes():
+            raise ValueError(f"workspace must be UINT8 [{operators.kv4_workspace_bytes()}] on {device}")
+        self.workspace = workspace
 
     def forward(self, x, positions, slots, cache, block_table, q_starts, kv_lens, axis_of=None):
         """x BF16 [tokens, K] -> BF16 [tokens, N], valid until the next call. positions INT64 [tokens] or [axes, tokens],

@@ -65,3 +65,15 @@ def test_refusals():
     for bad in (dict(page=24), dict(dim=32), dict(pages=0), dict(kv_heads=0)):
         with pytest.raises(ValueError):
             make_cache(**{**dict(pages=1, kv_heads=1, page=16, dim=64, device="cpu"), **bad})
+
+
+def test_layers_share_a_workspace():
+    shared = torch.zeros(64, dtype=torch.uint8)
+    first, ops = layer(workspace=shared)
+    second, _ = layer(workspace=shared)
+    assert first.workspace.data_ptr() == second.workspace.data_ptr() == shared.data_ptr()
+    forward(first)
+    assert dict(ops.calls)["kv4_attention"][5] is shared
+    for bad in (torch.zeros(63, dtype=torch.uint8), torch.zeros(64, dtype=torch.int8), torch.zeros(64, dtype=torch.uint8, device="meta")):
+        with pytest.raises(ValueError, match="workspace"):
+            layer(workspace=bad)
