@@ -464,9 +464,10 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       most = fabsf(most);
       most = max_abs_keep_nan(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fabsf(max_abs_keep_nan(most, __shfl_xor_sync(0xffffffffu, most, 2)));
-      const float scale = most > 0.f ? 32639.f / most : 0.f;             // 127 * 256 + 127
-      // a row with a NaN or an infinity is NaN as a whole
-      const float unit = most < INFINITY ? most * (1.f / 32639.f) * p.scale_log2 : __int_as_float(0x7fffffff);
+      // 127 * 256 + 127 steps; from 2^-100 on, so that a row of zeros or of the smallest numbers has a finite scale too
+      const float largest = fmaxf(most, 0x1p-100f), scale = 32639.f / largest;
+      // a row with a NaN or an infinity has NaN scores
+      const float unit = most < INFINITY ? largest * (1.f / 32639.f) * p.scale_log2 : __int_as_float(0x7fffffff);
       int digits_sum = 0;
 #pragma unroll
       for (int k = 0; k < kKWords; ++k) {
@@ -531,7 +532,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       const bool whole = first + kTile <= least && (info.w & ((1 << kParts) - 1)) == (1 << kParts) - 1;
       auto usable = [&](int t) { return (info.w >> (t >> 4)) & 1; };
 
-      // S^T = K Q^T, in units of key scale * query unit
+      // S^T = K Q^T, complete (query unit, then key scale: an integer sum times a key scale may leave FP32's range) before
+      // keys are hidden, so that hidden ones count for nothing whatever the unit is
       float s[kParts][kQ][4], top[kQ][2], vscale[kParts][2];
 #pragma unroll
       for (int n = 0; n < kQ; ++n) top[n][0] = top[n][1] = -INFINITY;
@@ -575,10 +577,14 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
             const float kscale = bf16_lo(key_pair);
             const int zero = __float2int_rn(bf16_hi(key_pair));
 #pragma unroll
-            for (int n = 0; n < kQ; ++n)
+            for (int n = 0; n < kQ; ++n) {
+              float x[2];
 #pragma unroll
-              for (int e = 0; e < 2; ++e)
-                s[mt][n][2 * r + e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]) * kscale;
+              for (int e = 0; e < 2; ++e) x[e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]);
+              const float2 score = __fmul2_rn(__fmul2_rn(make_float2(x[0], x[1]), make_float2(qscale[n][0], qscale[n][1])), make_float2(kscale, kscale));
+              s[mt][n][2 * r] = score.x;
+              s[mt][n][2 * r + 1] = score.y;
+            }
           }
       }
       if (!whole) {
@@ -609,7 +615,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         for (int e = 0; e < 2; ++e) {
           top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
           top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
-          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16)) * qscale[n][e];
+          top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16));
           grows |= top[n][e] > m[n][e] + 8.f;
         }
       // The maximum follows only when it has grown by more than 2^8 (weights up to 256 fit), so that the output is rarely
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
           float x[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float weight = fast_exp2(fmaf(s[mt][n][j], qscale[n][j % 2], base[n][j % 2]));
+            const float weight = fast_exp2(s[mt][n][j] + base[n][j % 2]);
             sum[n][j % 2] += weight;
             x[j] = weight * scale[j / 2];
           }
