@@ -6,8 +6,8 @@
 //   unpack warps   codes from global memory (a half-step ahead, in registers) -> BF16 code - zero, exact small integers,
 //                  into the 128-byte-swizzled operand tiles; scales beside them as FP32
 //   MMA warp       S = Q K^T (Q from TMEM where it has room, from shared memory for dim 128), O += P V (P from TMEM)
-//   softmax warps  32 rows each: S * key scale, running maximum and sum, weights * value scale rounded to BF16
-//                  into the columns of S. The output is scaled only when a row's maximum has grown by more than 2^8.
+//   softmax warps  32 rows each: S * key scale (times the softmax scale), running maximum and sum, weights * value scale
+//                  rounded to BF16 into the columns of S. The output is scaled only when a row's maximum has grown by more than 2^8.
 // The components of a word come out of the unpacking as 0 4 1 5 2 6 3 7; the queries are stored in that order and the
 // output is put back.
 //
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.scale_log2;
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
           grows |= top[r] > m[r] + 8.f;
         }
         if (__any_sync(0xffffffffu, grows)) {
@@ -417,7 +417,6 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
         }
         fine = warp_wait(&bar_scale_v[slot], slot_parity, &abort_flag);
         if (!fine) break;
-        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
         float2 base2[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) base2[r].x = base2[r].y = m[r] == -INFINITY ? 0.f : -m[r];
@@ -430,7 +429,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const uint32_t* at = &s[h][r / 2][4 * i + 2 * (r & 1)];
-              float2 x = __ffma2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), scale2, base2[r]);
+              float2 x = __fadd2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), base2[r]);
               x = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
               sum2[r] = __fadd2_rn(sum2[r], x);
               x = __fmul2_rn(x, v);
@@ -584,7 +583,9 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           const int row = kPassRows * i + lane_row;
           const float zero = 128.f + bf16_hi(now_pairs[i]);
           const uint32_t zeros = pack2(zero, zero);
-          if (lane_piece == 0) (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]);
+          // the softmax scale comes with the keys': a score and the maximum are then one rounded number, and their difference
+          // is exact where the score is the maximum, however large
+          if (lane_piece == 0) (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]) * (side ? 1.f : p.scale_log2);
           uint32_t words[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
 #pragma unroll
           for (int bit = 1; kDim == 256 && bit < 4; bit *= 2)

@@ -88,7 +88,7 @@ def test_nan_queries_that_see_nothing_are_zeros(ops, workspace, dim):
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("sequences", [[(1, 70), (1, 300)], [(3, 70), (20, 300)]])
+@pytest.mark.parametrize("sequences", [[(1, 70), (1, 300)], [(3, 70), (20, 300)], [(3, 70), (100, 300)]])
 def test_a_key_at_the_end_of_its_range_takes_all_the_weight(ops, workspace, dim, sequences):
     """An infinite key component is held as 8.5e37. Queries of up to 2.5 make products of up to 2.2e38, within FP32: the rows
     that see the key answer with its value, the others as if it were not there."""
@@ -110,3 +110,23 @@ def test_a_key_at_the_end_of_its_range_takes_all_the_weight(ops, workspace, dim,
         first = int(case.starts[b]) + max(0, place - (keys - rows))
         diff = (out[first:int(case.starts[b + 1])].double() - value).abs()
         assert bool((diff <= 2.0 ** -8 * value.abs()).all())            # one rounding: weight 1 and its value's scale are exact
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("sequences", [[(1, 70), (9, 300)], [(100, 300), (80, 80), (30, 1500)]])
+def test_scores_far_beyond_2_to_the_24(ops, workspace, dim, sequences):
+    """Scores of about 1e12, of which an FP32 number holds no fraction: one key takes all the weight, and the output is finite.
+    (The bound says no more here: a score's own rounding is larger than the distance between keys.)"""
+    case = Case(sequences, 4, 2, dim, 16, seed=dim, magnitude=1e5)
+    case.q *= 1e6
+    out = run_and_check(ops, workspace, case).cpu().double()
+    held = ref.values(case.cache, dim)
+    for b, (rows, keys) in enumerate(sequences):
+        ids = case.table[b, : -(-keys // 16)].long()
+        values = held[ids, 1].permute(1, 0, 2, 3).flatten(1, 2)[:, :keys]                  # [heads, keys, dim]
+        start = int(case.starts[b])
+        for h in range(4):
+            low, high = values[h // 2].amin(0), values[h // 2].amax(0)
+            got = out[start:start + rows, h]
+            room = 2.0 ** -8 * torch.maximum(low.abs(), high.abs())
+            assert bool((got >= low - room).all()) and bool((got <= high + room).all())
