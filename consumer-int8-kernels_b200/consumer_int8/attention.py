@@ -3,7 +3,7 @@
     quantize_rows -> fused_channel_mm (QKV) -> qk_norm_rope -> kv4_append -> kv4_attention -> quantize_rows
     -> fused_channel_mm (output projection)
 
-Seven launches (eight or nine when prompts are among the rows) on the current stream over buffers allocated once, so a
+A clear and seven launches (eight or nine when prompts are among the rows) on the current stream over buffers allocated once, so a
 call can be captured in a CUDA graph; lengths, pages, slots and positions are read on the device, and a replay follows
 their values. The cache is a tensor of the caller's (:func:`make_cache`), as is the bookkeeping of its pages.
 """
@@ -74,7 +74,7 @@ class Kv4AttentionLayer:
         """x BF16 [tokens, K] -> BF16 [tokens, N], valid until the next call. positions INT64 [tokens] or [axes, tokens],
         slots INT64 [tokens] (where each row's key and value go, negative: padding); block_table INT32 [batch, width],
         q_starts INT32 [batch + 1] and kv_lens INT32 [batch] as ``kv4_attention`` takes them: a sequence's length counts
-        the rows of this call."""
+        the rows of this call. Rows of no sequence (padding) come out as the product of zeros."""
         tokens = x.shape[0]
         if tokens > self.out.shape[0]:
             raise ValueError(f"{tokens} rows: the layer's buffers hold {self.out.shape[0]}")
@@ -82,6 +82,10 @@ class Kv4AttentionLayer:
             return self.out[:0]
         ops = self.ops
         codes, scales, qkv = self.codes[:tokens], self.row_scales[:tokens], self.qkv[:tokens]
+        attended = self.attended[:tokens]
+        # rows of no sequence are left alone by the attention: without this they would be an earlier call's. Ahead of the
+        # launches, which follow one another without a gap
+        attended.zero_()
         ops.quantize_rows(x, codes, scales)
         ops.fused_channel_mm(codes, self.w_qkv, scales, self.qkv_scale, qkv)
         heads = qkv.view(tokens, -1, self.dim)
@@ -96,7 +100,6 @@ class Kv4AttentionLayer:
             ops.kv4_append(q, k, v, cos_sin, at, axis_of, slots, q, cache, self.adjacent)
         else:
             ops.kv4_append(None, k, v, None, None, None, slots, None, cache, False)
-        attended = self.attended[:tokens]
         ops.kv4_attention(q, cache, block_table, q_starts, kv_lens, self.workspace, attended, self.scale)
         flat = self.attended_codes[:tokens]
         ops.quantize_rows(attended.view(tokens, -1), flat, scales)
