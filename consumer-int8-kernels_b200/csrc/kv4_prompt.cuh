@@ -62,6 +62,11 @@ struct Kv4PromptParams {
 constexpr int kKv4ScaleSlots = 8;
 constexpr int kKv4MarkSlots = 2 * kKv4ScaleSlots;
 
+// Outputs are sums of weights (up to 2^8) times values (up to 2^127) over up to 2^30 keys until they are divided by the weights'
+// sum. They are kept in units of 2^40, as the values' scales are: 2^125 at most, and the least scale, 2^-66, leaves weights down
+// to 2^-20 normal.
+constexpr float kKv4ValueUnit = 0x1p40f;
+
 __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n, bool b_transposed) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_transposed ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
@@ -479,7 +484,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           }
         }
       } else {
-        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        const float inverse = sum == 0.f ? 0.f : kKv4ValueUnit / sum;
         uint16_t* dst = p.out + (static_cast<int64_t>(seq.start + token) * p.q_heads + head * group + row - token * group) * kDim;
 #pragma unroll 1
         for (int c = 0; c < kDim; c += 32) {
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
           const uint32_t zeros = pack2(zero, zero);
           // the softmax scale comes with the keys': a score and the maximum are then one rounded number, and their difference
           // is exact where the score is the maximum, however large
-          if (lane_piece == 0) (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]) * (side ? 1.f : p.scale_log2);
+          if (lane_piece == 0) (side ? scale_v : scale_k)[slot][row] = bf16_lo(now_pairs[i]) * (side ? 1.f / kKv4ValueUnit : p.scale_log2);
           uint32_t words[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
 #pragma unroll
           for (int bit = 1; kDim == 256 && bit < 4; bit *= 2)
@@ -765,7 +770,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const Kv4PromptPar
       all += weight * sum;
       x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
     }
-    const float inverse = all == 0.f ? 0.f : 1.f / all;
+    const float inverse = all == 0.f ? 0.f : kKv4ValueUnit / all;
     const int r = first_row + row, token = p.group.quotient(r);
     uint16_t* dst = p.out + (static_cast<int64_t>(seq.start + token) * p.q_heads + head * group + r - token * group) * kDim + column;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(x.x * inverse, x.y * inverse), pack2(x.z * inverse, x.w * inverse));

@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   __shared__ Kv4Piece pieces[2 * kWarps];
   __shared__ Kv4Piece shared_units[2];                   // sequences shared with the CTA before [0] and behind [1]
   __shared__ float piece_m[2 * kWarps][kRows], piece_l[2 * kWarps][kRows], group_m[2 * kWarps][kRows], group_l[2 * kWarps][kRows];
-  __shared__ float weights[2 * kWarps][kRows], inverse_sums[kRows];
+  __shared__ float weights[2 * kWarps][kRows];
   __shared__ int comes_last[2];
   const Kv4AttendParams& p = params.a;
   const int thread = threadIdx.x, warp = thread / 32, lane = thread % 32, g = lane / 4, c = lane % 4;
@@ -402,7 +402,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   uint32_t ones;                                         // kept in a register: an immediate would cost a second instruction
   asm volatile("mov.b32 %0, 0x64006400;" : "=r"(ones));
 
-  // Leaves this warp's maximum, sum (in piece_m, piece_l) and output of every row.
+  // Leaves this warp's maximum, sum (in piece_m, piece_l) and output of every row. An output is divided by its sum before it
+  // leaves the unit it was summed in, here and wherever pieces are joined: sums of large values have no place in FP32.
   auto write_piece = [&](int piece, float* dst) {
     const float unit = 1.f / value_unit;                 // a power of two
 #pragma unroll
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = 8 * n + 2 * c + e;
+        const float inverse = sum[n][e] == 0.f ? 0.f : unit / sum[n][e];
         if (g == 0) {
           piece_m[piece][row] = m[n][e];
           piece_l[piece][row] = sum[n][e];
@@ -417,8 +419,8 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
 #pragma unroll
         for (int k = 0; k < kVWords; ++k) {
           float4* to = reinterpret_cast<float4*>(dst + row * kDim + 8 * (kVWords * g + k));
-          to[0] = make_float4(o[4 * k][n][e] * unit, o[4 * k + 1][n][e] * unit, o[4 * k + 2][n][e] * unit, o[4 * k + 3][n][e] * unit);
-          to[1] = make_float4(o[4 * k][n][2 + e] * unit, o[4 * k + 1][n][2 + e] * unit, o[4 * k + 2][n][2 + e] * unit, o[4 * k + 3][n][2 + e] * unit);
+          to[0] = make_float4(o[4 * k][n][e] * inverse, o[4 * k + 1][n][e] * inverse, o[4 * k + 2][n][e] * inverse, o[4 * k + 3][n][e] * inverse);
+          to[1] = make_float4(o[4 * k][n][2 + e] * inverse, o[4 * k + 1][n][2 + e] * inverse, o[4 * k + 2][n][2 + e] * inverse, o[4 * k + 3][n][2 + e] * inverse);
         }
       }
   };
@@ -767,16 +769,16 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     const uint32_t mask = group_mask(piece);
     float most = -INFINITY, all = 0.f;
     for (uint32_t rest = mask; rest; rest &= rest - 1) most = fmaxf(most, piece_m[__ffs(rest) - 1][row]);
+    auto part = [&](int other) {
+      const float l = piece_l[other][row];
+      return l == 0.f ? 0.f : fast_exp2(piece_m[other][row] - most) * l;     // 0: saw no key (a NaN score makes the sum NaN, which is kept)
+    };
+    for (uint32_t rest = mask; rest; rest &= rest - 1) all += part(__ffs(rest) - 1);
     if (piece == __ffs(mask) - 1) {
-      for (uint32_t rest = mask; rest; rest &= rest - 1) {
-        const int other = __ffs(rest) - 1;
-        const float l = piece_l[other][row];
-        all += l == 0.f ? 0.f : fast_exp2(piece_m[other][row] - most) * l;   // 0: saw no key (a NaN score makes the sum NaN, which is kept)
-      }
       group_m[piece][row] = most;
       group_l[piece][row] = all;
     }
-    weights[piece][row] = piece_l[piece][row] == 0.f ? 0.f : fast_exp2(piece_m[piece][row] - most);
+    weights[piece][row] = all == 0.f ? 0.f : part(piece) / all;
   }
   __syncthreads();
   auto write_out = [&](const Kv4Piece& unit, int row, int column, const float4& x) {
@@ -804,15 +806,13 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       const float4 y = *reinterpret_cast<const float4*>(from + row * kDim + column);
       x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
     }
-    const float all = group_l[piece][row];
     if (unit.starts && (mask & ends)) {
-      const float inverse = all == 0.f ? 0.f : 1.f / all;
-      write_out(unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+      write_out(unit, row, column, x);
     } else {
       float* slot = params.slots + (2ll * blockIdx.x + (unit.starts ? 1 : 0)) * Cfg::kPieceFloats;
       if (column == 0) {
         slot[row] = group_m[piece][row];
-        slot[kRows + row] = all;
+        slot[kRows + row] = group_l[piece][row];
         if (row == 0) shared_units[unit.starts ? 1 : 0] = unit;
       }
       *reinterpret_cast<float4*>(slot + 2 * kRows + row * kDim + column) = x;
@@ -851,13 +851,14 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
       for (int d = 16; d; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
       for (int i = lane; i < count_ctas; i += 32) {
         const float part_sum = __ldcg(slot_of(i) + kRows + row);
-        const float weight = part_sum == 0.f ? 0.f : fast_exp2(__ldcg(slot_of(i) + row) - most);
-        cta_weights[i * kRows + row] = weight;
-        all += weight * part_sum;
+        const float part = part_sum == 0.f ? 0.f : fast_exp2(__ldcg(slot_of(i) + row) - most) * part_sum;
+        cta_weights[i * kRows + row] = part;
+        all += part;
       }
 #pragma unroll
       for (int d = 16; d; d /= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
-      if (lane == 0) inverse_sums[row] = all == 0.f ? 0.f : 1.f / all;
+      if (all != 0.f)
+        for (int i = lane; i < count_ctas; i += 32) cta_weights[i * kRows + row] /= all;
     }
     __syncthreads();
     for (int e = thread; e < rows * (kDim / 4); e += kThreads) {
@@ -869,8 +870,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         const float4 y = __ldcg(reinterpret_cast<const float4*>(slot_of(i) + 2 * kRows + row * kDim + column));
         x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;
       }
-      const float inverse = inverse_sums[row];
-      write_out(unit, row, column, make_float4(x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse));
+      write_out(unit, row, column, x);
     }
     __syncthreads();
   }
