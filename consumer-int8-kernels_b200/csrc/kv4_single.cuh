@@ -22,8 +22,8 @@
 //        queries' own rounding. The sums, less zero * sum of q, stay exact until the key's scale is applied in FP32.
 //   O^T  FP16 (m16n8k16): a mask-and-or gives 1024 + code or 1024 + 16 * code for two tokens, one packed FMA the exact
 //        small integer code - zero (not zero points taken out of the sum afterwards: a sum over the whole history
-//        would cancel). The weights carry the values' scales, relative to the largest scale so far, which keeps them
-//        within FP16: full precision down to 2^-21 of the largest, 2^-11 relative rounding.
+//        would cancel). The weights carry the values' scales, relative to the largest scale that the row has seen so far, which
+//        keeps them within FP16: 2^-11 relative rounding down to 2^-21 of the largest, multiples of 2^-31 of it below.
 // Maxima, sums, scores and outputs are FP32.
 #pragma once
 #include "kv4_attention.cuh"
@@ -386,7 +386,12 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   float o[4 * kVWords][kQ][4];
   float m[kQ][2], sum[kQ][2], qscale[kQ][2];
   int qsum[kQ][2];
-  float most_scale = 0.f, value_unit = 1.f;              // power of two above the values' scales so far; 128 / it
+  // 128 / the power of two above the values' scales that the row has seen so far (a row of its own: large values that are hidden
+  // from it must not push its weights out of FP16); before the first scale above 0 2^118, which a weight may be multiplied with.
+  // Powers of two, so two rows' fit a register as BF16 numbers.
+  uint32_t value_units[kQ];
+  constexpr uint32_t kFirstUnits = 0x7a807a80u;
+  auto value_unit = [&](int n, int e) { return e ? bf16_hi(value_units[n]) : bf16_lo(value_units[n]); };
   int limit[kQ][2];
   uint32_t q[kKWords][kQ][4];                            // high digits (even, odd components of a word), low digits
   int cur_b = 0, cur_head = 0, cur_block = 0, cur_tile = 0, cur_rows = 0, cur_start = 0, cur_keys = 0, first_tile = 0;
@@ -405,13 +410,12 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   // Leaves this warp's maximum, sum (in piece_m, piece_l) and output of every row. An output is divided by its sum before it
   // leaves the unit it was summed in, here and wherever pieces are joined: sums of large values have no place in FP32.
   auto write_piece = [&](int piece, float* dst) {
-    const float unit = 1.f / value_unit;                 // a power of two
 #pragma unroll
     for (int n = 0; n < kQ; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = 8 * n + 2 * c + e;
-        const float inverse = sum[n][e] == 0.f ? 0.f : unit / sum[n][e];
+        const float inverse = sum[n][e] == 0.f ? 0.f : 1.f / value_unit(n, e) / sum[n][e];   // the unit is a power of two
         if (g == 0) {
           piece_m[piece][row] = m[n][e];
           piece_l[piece][row] = sum[n][e];
@@ -441,8 +445,6 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     cur_start = s.start;
     cur_keys = kv4_block_keys(s, p.group, kRows, cur_block);
     least = 0x7fffffff;
-    most_scale = 0.f;
-    value_unit = 1.f;
 #pragma unroll
     for (int n = 0; n < kQ; ++n) {
       const int row = cur_block * kRows + 8 * n + g, row_token = p.group.quotient(row);
@@ -502,6 +504,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         m[n][e] = -INFINITY;
         sum[n][e] = 0.f;
       }
+      value_units[n] = kFirstUnits;
 #pragma unroll
       for (int k = 0; k < 4 * kVWords; ++k)
 #pragma unroll
@@ -583,7 +586,11 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
               float x[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) x[e] = static_cast<float>(high[u][n][2 * r + e] * 256 + low[u][n][2 * r + e] - zero * qsum[n][e]);
-              const float2 score = __fmul2_rn(__fmul2_rn(make_float2(x[0], x[1]), make_float2(qscale[n][0], qscale[n][1])), make_float2(kscale, kscale));
+              // two to an instruction, but for dim 256 with sixteen rows, whose registers are all taken (174 us packed, 159 not, for
+              // 32 sequences of 8192 keys, 12 query heads on each of 4 key heads; 16 on 4 of dim 128 72 packed, 74 not)
+              float2 score = make_float2(x[0] * qscale[n][0] * kscale, x[1] * qscale[n][1] * kscale);
+              if constexpr (kDim * kQ < 512)
+                score = __fmul2_rn(__fmul2_rn(make_float2(x[0], x[1]), make_float2(qscale[n][0], qscale[n][1])), make_float2(kscale, kscale));
               s[mt][n][2 * r] = score.x;
               s[mt][n][2 * r + 1] = score.y;
             }
@@ -606,11 +613,11 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) top[n][j % 2] = fmaxf(top[n][j % 2], s[mt][n][j]);
-      float lane_scale = 0.f;
+      float tile_scale = 0.f;
 #pragma unroll
-      for (int mt = 0; mt < kParts; ++mt) lane_scale = fmaxf(lane_scale, fmaxf(vscale[mt][0], vscale[mt][1]));
-      const float tile_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lane_scale)));
-      bool grows = tile_scale > most_scale;
+      for (int mt = 0; mt < kParts; ++mt) tile_scale = fmaxf(tile_scale, fmaxf(vscale[mt][0], vscale[mt][1]));
+      tile_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tile_scale)));
+      bool grows = !whole;                               // rows see different scales there: looked at below
 #pragma unroll
       for (int n = 0; n < kQ; ++n)
 #pragma unroll
@@ -618,22 +625,31 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
           top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 4));
           top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 8));
           top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], 16));
-          grows |= top[n][e] > m[n][e] + 8.f;
+          grows |= top[n][e] > m[n][e] + 8.f || tile_scale * value_unit(n, e) > 128.f;
         }
       // The maximum follows only when it has grown by more than 2^8 (weights up to 256 fit), so that the output is rarely
       // scaled again.
       if (__any_sync(0xffffffffu, grows)) {
-        float turn = 1.f;
-        if (tile_scale > most_scale) {
-          most_scale = __uint_as_float((__float_as_uint(tile_scale) + 0x007fffffu) & 0xff800000u);
-          const float next = 128.f / most_scale;
-          turn = next / value_unit;
-          value_unit = next;
-        }
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+            float seen = tile_scale, turn = 1.f;         // the largest of the values' scales that the row sees
+            if (!whole) {
+              seen = 0.f;
+#pragma unroll
+              for (int mt = 0; mt < kParts; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                  if (s[mt][n][2 * r + e] != -INFINITY) seen = fmaxf(seen, vscale[mt][r]);
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) seen = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, d));
+            }
+            if (seen * value_unit(n, e) > 128.f) {
+              const float unit = 128.f / __uint_as_float((__float_as_uint(seen) + 0x007fffffu) & 0xff800000u);
+              turn = unit / value_unit(n, e);
+              value_units[n] = __byte_perm(value_units[n], __float_as_uint(unit), e ? 0x7610 : 0x3276);
+            }
             const float next = fmaxf(m[n][e], top[n][e]);
             float keep = next == -INFINITY ? 1.f : fast_exp2(m[n][e] - next);
             m[n][e] = next;
@@ -655,19 +671,21 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
         for (int e = 0; e < 2; ++e) base[n][e] = m[n][e] == -INFINITY ? 0.f : -m[n][e];
 #pragma unroll
       for (int mt = 0; mt < kParts; ++mt) {
-        const float scale[2] = {vscale[mt][0] * value_unit, vscale[mt][1] * value_unit};
 #pragma unroll
-        for (int n = 0; n < kQ; ++n) {
-          float x[4];
+        for (int n = 0; n < kQ; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float weight = fast_exp2(s[mt][n][j] + base[n][j % 2]);
-            sum[n][j % 2] += weight;
-            x[j] = weight * scale[j / 2];
+          for (int r = 0; r < 2; ++r) {
+            float weight[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              weight[e] = fast_exp2(s[mt][n][2 * r + e] + base[n][e]);
+              sum[n][e] += weight[e];
+            }
+            // in this order: a hidden key's weight is 0, and its scale times the row's unit may leave FP32's range
+            const float2 x = __fmul2_rn(__fmul2_rn(make_float2(weight[0], weight[1]), make_float2(value_unit(n, 0), value_unit(n, 1))),
+                                        make_float2(vscale[mt][r], vscale[mt][r]));
+            w[mt][n][r] = transpose8x8(pack_f16(x.x, x.y));
           }
-          w[mt][n][0] = transpose8x8(pack_f16(x[0], x[1]));
-          w[mt][n][1] = transpose8x8(pack_f16(x[2], x[3]));
-        }
       }
       // O^T += V^T P^T
 #pragma unroll
@@ -711,14 +729,13 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
     if (info.w >> kParts & 1) {                          // the last tile of these rows
       add_sums();
       if (first_tile == 0) {
-        const float unit = 1.f / value_unit;
 #pragma unroll
         for (int n = 0; n < kQ; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int row = cur_block * kRows + 8 * n + 2 * c + e;
             if (row >= cur_rows) continue;
-            const float inverse = sum[n][e] == 0.f ? 0.f : unit / sum[n][e];
+            const float inverse = sum[n][e] == 0.f ? 0.f : 1.f / value_unit(n, e) / sum[n][e];
             const int row_token = p.group.quotient(row);
             uint16_t* dst = p.out + (static_cast<int64_t>(cur_start + row_token) * p.q_heads + cur_head * group + row - row_token * group) * kDim;
 #pragma unroll

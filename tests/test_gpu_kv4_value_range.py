@@ -5,9 +5,9 @@ Bounds as derived beside the attention's own tests."""
 import pytest
 import torch
 
-from gpu_common import DEV
+from gpu_common import DEV, device_status
 from oracle import kv4_ref as ref
-from test_gpu_kv4_attention import Case, run_and_check
+from test_gpu_kv4_attention import Case, run_and_check, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,42 @@ def test_the_smallest_values(ops, workspace, dim, sequences):
         for key in range(keys):
             set_value(case, b, key, torch.randn(2, dim, generator=torch.Generator().manual_seed(key)) * 1e-20)
     run_and_check(ops, workspace, case)
+
+
+def small_weights(case):
+    """What the streaming kernel's FP16 weights lose beside the bound's relative 2^-11: they are multiples of 2^-24 in a unit in which
+    the largest value scale that the row sees is between 64 and 128. A weight is off by at most half of that, 2^-25 * largest / 64,
+    a component by 15 times that for each key, and the weights' sum that it is divided by is at least 1. [tokens, q_heads, 1]"""
+    _, pairs = ref.rows(case.cache, case.dim)
+    lost = torch.zeros(case.q.shape[0], case.kv_heads, 1, dtype=torch.float64)
+    for b, keys in enumerate(case.lens.tolist()):
+        ids = case.table[b, : -(-keys // case.page)].long()
+        scales = pairs[ids, 1, :, :, 0].permute(1, 0, 2).flatten(1)[:, :keys].double()     # [heads, keys]
+        start, end = int(case.starts[b]), int(case.starts[b + 1])
+        for row in range(start, end):
+            count = keys - (end - start) + row - start + 1
+            if count > 0:
+                lost[row, :, 0] = scales[:, :count].amax(1) * count * 15 * 2.0 ** -31
+    return lost.repeat_interleave(case.q.shape[1] // case.kv_heads, 1)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e9, float("inf")])
+@pytest.mark.parametrize("q_heads,kv_heads", [(4, 2), (2, 2), (24, 2)])
+def test_large_values_that_are_hidden_from_a_row(ops, workspace, dim, size, q_heads, kv_heads):
+    """New rows do not see the rows behind them: those before one with very large values answer as if it were not there. The large
+    ones stand first, in the middle and last among the new rows, and alone behind a long prefix whose parts are joined."""
+    sequences = [(5, 40), (9, 130), (2, 2), (4, 1500), (1, 20), (30, 63), (90, 130)]
+    case = Case(sequences, q_heads, kv_heads, dim, 16, seed=dim + q_heads)
+    large = {0: [4], 1: [3, 8], 2: [1], 3: [2], 5: [15, 29], 6: [40]}
+    for b, rows in large.items():
+        n, keys = sequences[b]
+        for row in rows:
+            x = torch.randn(kv_heads, dim, generator=torch.Generator().manual_seed(row)).clamp(-3, 3)
+            set_value(case, b, keys - n + row, x * size)
+    out = torch.full(case.q.shape, float("nan"), dtype=torch.bfloat16, device=DEV)
+    ops.kv4_attention(*case.device(), workspace, out, case.scale)
+    want, spread, reach = case.want()
+    bound = tolerance(want, spread, reach) + small_weights(case)
+    assert bool(((out.cpu().double() - want).abs() <= bound).all())
+    assert device_status(ops) == 0
