@@ -433,6 +433,12 @@ bool overlap(const Heads& a, const void* data, int64_t bytes) {
   const int64_t first = reinterpret_cast<intptr_t>(a.data), second = reinterpret_cast<intptr_t>(data);
   return first < second + bytes && second < first + 2 * ((a.tokens - 1) * a.stride + a.heads * a.dim);
 }
+bool overlap(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
+  if (!bytes_a || !bytes_b) return false;
+  const int64_t first = reinterpret_cast<intptr_t>(a), second = reinterpret_cast<intptr_t>(b);
+  return first < second + bytes_b && second < first + bytes_a;
+}
+bool overlap(const void* a, int64_t bytes_a, const Tensor& b) { return overlap(a, bytes_a, b.data_ptr(), b.numel() * b.element_size()); }
 bool same_rows(const Heads& a, const Heads& b) { return a.data == b.data && a.stride == b.stride; }
 
 struct Rotation {
@@ -468,6 +474,16 @@ Rotation rotation_of(const OptionalTensor& cos_sin, const OptionalTensor& positi
   r.rotary = static_cast<int>(cos_sin->size(1));
   r.axes = static_cast<int>(axes);
   return r;
+}
+
+// Whether an output shares memory with what says where and how far heads are turned.
+bool overlap(const Heads& out, const Rotation& r) {
+  return overlap(out, r.cos_sin, 4ll * r.table_rows * r.rotary) || overlap(out, r.positions, r.positions ? 8 * r.axes * out.tokens : 0) ||
+         overlap(out, r.axis_of, r.axis_of ? 2ll * r.rotary : 0);
+}
+bool overlap(const void* out, int64_t bytes, const Rotation& r, int64_t tokens) {
+  return overlap(out, bytes, r.cos_sin, 4ll * r.table_rows * r.rotary) ||
+         overlap(out, bytes, r.positions, r.positions ? 8 * r.axes * tokens : 0) || overlap(out, bytes, r.axis_of, r.axis_of ? 2ll * r.rotary : 0);
 }
 
 struct Cache {
@@ -507,6 +523,7 @@ void boxed_qk_norm_rope(StableIValue* stack, uint64_t, uint64_t) {
                       !overlap(ok, hq) && !overlap(oq, ok),
                   "An output may be its own input and must not overlap anything else");
   const Rotation r = rotation_of(cos_sin, positions, axis_of, hk, device);
+  STD_TORCH_CHECK(!overlap(oq, r) && !overlap(ok, r), "Outputs must not overlap cos_sin, positions or axis_of");
   torch::stable::accelerator::DeviceGuard guard(device);
   launched(ci8_qk_norm_rope(hq.data, hq.stride, hk.data, hk.stride, q_weight.has_value() ? q_weight->data_ptr() : nullptr,
                             k_weight.has_value() ? k_weight->data_ptr() : nullptr, r.cos_sin, r.table_rows, r.rotary, r.positions, r.axes,
@@ -541,6 +558,9 @@ void boxed_kv4_append(StableIValue* stack, uint64_t, uint64_t) {
                     "q_out may be q and must not overlap anything else");
   }
   const Rotation r = rotation_of(cos_sin, positions, axis_of, hk, device);
+  STD_TORCH_CHECK(!overlap(oq, r) && !overlap(oq, slots.data_ptr(), 8 * hk.tokens) && !overlap(c.data, c.bytes, r, hk.tokens) &&
+                      !overlap(c.data, c.bytes, slots),
+                  "q_out and cache must not overlap cos_sin, positions, axis_of or slots");
   torch::stable::accelerator::DeviceGuard guard(device);
   launched(ci8_kv4_append(hq.data, hq.stride, hk.data, hk.stride, hv.data, hv.stride, r.cos_sin, r.table_rows, r.rotary, r.positions,
                           r.axes, r.axis_of, static_cast<const int64_t*>(slots.data_ptr()), oq.data, oq.stride, c.data, c.pages, c.page,
@@ -587,6 +607,8 @@ void boxed_kv4_attention(StableIValue* stack, uint64_t, uint64_t) {
                       !overlap(hq, workspace.data_ptr(), workspace.numel()) && !overlap(ho, block_table.data_ptr(), 4 * block_table.numel()) &&
                       !overlap(ho, q_starts.data_ptr(), 4 * q_starts.numel()) && !overlap(ho, kv_lens.data_ptr(), 4 * kv_lens.numel()),
                   "out and workspace must not overlap anything else");
+  for (const Tensor* t : {&cache, &block_table, &q_starts, &kv_lens})
+    STD_TORCH_CHECK(!overlap(workspace.data_ptr(), workspace.numel(), *t), "out and workspace must not overlap anything else");
   torch::stable::accelerator::DeviceGuard guard(device);
   launched(ci8_kv4_attention(hq.data, hq.stride, c.data, static_cast<const int32_t*>(block_table.data_ptr()),
                              static_cast<const int32_t*>(q_starts.data_ptr()), static_cast<const int32_t*>(kv_lens.data_ptr()),
