@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   // 128 / the power of two above the values' scales that the row has seen so far (a row of its own: large values that are hidden
   // from it must not push its weights out of FP16); before the first scale above 0 2^118, which a weight may be multiplied with.
   // Powers of two, so two rows' fit a register as BF16 numbers.
-  uint32_t value_units[kQ];
+  uint32_t value_units[kQ] = {};
   constexpr uint32_t kFirstUnits = 0x7a807a80u;
   auto value_unit = [&](int n, int e) { return e ? bf16_hi(value_units[n]) : bf16_lo(value_units[n]); };
   int limit[kQ][2];
