@@ -602,7 +602,7 @@ void boxed_kv4_attention(StableIValue* stack, uint64_t, uint64_t) {
                   "Expected INT32 block_table [batch, width] (pages of 2^30 tokens at most), q_starts [batch + 1] and kv_lens [batch]");
   STD_TORCH_CHECK(workspace.numel() >= ci8_kv4_workspace_bytes() && address(workspace) % 16 == 0,
                   "The attention workspace is too small or not aligned");
-  STD_TORCH_CHECK(scale > 0 && scale < 3.0e38, "The softmax scale must be positive and finite");
+  STD_TORCH_CHECK(scale > 0 && scale < 2.3e38, "The softmax scale must be positive, finite and below 2.3e38");
   STD_TORCH_CHECK(!overlap(ho, hq) && !overlap(ho, c.data, c.bytes) && !overlap(ho, workspace.data_ptr(), workspace.numel()) &&
                       !overlap(hq, workspace.data_ptr(), workspace.numel()) && !overlap(ho, block_table.data_ptr(), 4 * block_table.numel()) &&
                       !overlap(ho, q_starts.data_ptr(), 4 * q_starts.numel()) && !overlap(ho, kv_lens.data_ptr(), 4 * kv_lens.numel()),

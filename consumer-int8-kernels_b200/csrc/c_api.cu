@@ -1421,7 +1421,7 @@ int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, cons
                       int q_heads, int kv_heads, int dim, float scale, ci8_stream_t stream) {
   const int shift = kv4_page_shift(page);
   if (tokens < 0 || batch < 0 || width < 0 || pages < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads > kKv4MaxHeads ||
-      q_heads % kv_heads || !kv4_dim(dim) || shift < 0 || !(scale > 0.f) || !(scale < 3.0e38f))
+      q_heads % kv_heads || !kv4_dim(dim) || shift < 0 || !(scale > 0.f) || !(scale < 2.3e38f))
     return kInvalid;
   if (tokens == 0 || batch == 0) return 0;
   if (!kv4_row_source(q, q_stride, tokens, q_heads, dim) || (pages > 0 && !cache) || !aligned(cache, 16) || (width > 0 && !block_table) ||

@@ -269,9 +269,10 @@ long long ci8_kv4_workspace_bytes(void);
  * ascending) of q and out, and the first kv_lens[b] (INT32) tokens of the pages block_table[b] (INT32 [batch, width])
  * names, the last of which are its own rows' (already appended): row i of n sees the first kv_lens[b] - n + i + 1
  * tokens. out = softmax(scale * q k^T) v, BF16 [tokens, q_heads, dim] contiguous; q_heads is a multiple of kv_heads,
- * scale > 0, width * page at most 2^30. Rows that see nothing are zeros; rows of no sequence are left as they were. Lengths
- * are cut to the table's width; tokens of a page number outside the cache are not seen (status bit 3), and entries behind a
- * sequence's last page are not read. All lengths are read on the device, so a captured call follows their values. */
+ * 0 < scale < 2.3e38 (times log2 e it has to be an FP32 number), width * page at most 2^30. Rows that see nothing are zeros;
+ * rows of no sequence are left as they were. Lengths are cut to the table's width; tokens of a page number outside the cache are
+ * not seen (status bit 3), and entries behind a sequence's last page are not read. All lengths are read on the device, so a
+ * captured call follows their values. */
 int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, const int32_t* block_table, const int32_t* q_starts,
                       const int32_t* kv_lens, void* workspace, void* out, int tokens, int batch, int width, int pages, int page,
                       int q_heads, int kv_heads, int dim, float scale, ci8_stream_t stream);
