@@ -3,9 +3,9 @@
     quantize_rows -> fused_channel_mm (QKV) -> qk_norm_rope -> kv4_append -> kv4_attention -> quantize_rows
     -> fused_channel_mm (output projection)
 
-A clear and seven launches (eight or nine when prompts are among the rows) on the current stream over buffers allocated once, so a
-call can be captured in a CUDA graph; lengths, pages, slots and positions are read on the device, and a replay follows
-their values. The cache is a tensor of the caller's (:func:`make_cache`), as is the bookkeeping of its pages.
+A clear and seven launches (eight or nine when prompts are among the rows) on the current stream over buffers allocated
+once, so a call can be captured in a CUDA graph; lengths, pages, slots and positions are read on the device, and a
+replay follows their values. The cache is a tensor of the caller's (:func:`make_cache`), as is the bookkeeping of its pages.
 """
 
 from __future__ import annotations

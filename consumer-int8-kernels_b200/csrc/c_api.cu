@@ -956,8 +956,8 @@ int launch_kv4_prompt(const Kv4AttendParams& a, void* workspace, int most_rows, 
 // Sequences with few query rows (tokens times heads per key head) go to the kernel for generated tokens, the others to the
 // one for prompts; which they are is only known on the device, so each kernel passes over the other's. The one takes time
 // with every eight rows, the other with every 128 or 256. Measured (us, the one and the other): 64 sequences of 4096 keys,
-// 8 key heads of 128, 32 rows 230 and 548, 64 rows 470 and 550, 128 rows 660 and 483; 16 sequences, 4 heads of 256, 48 rows
-// 102 and 118, 120 rows 245 and 117; one sequence of 8192 keys, 64 rows 30 and 42, 128 rows 42 and 48. No sequence has more
+// 8 key heads of 128, 32 rows 234 and 548, 64 rows 435 and 550, 128 rows 660 and 485; 16 sequences, 4 heads of 256, 48 rows
+// 102 and 118, 120 rows 245 and 117; one sequence of 8192 keys, 64 rows 32 and 42, 128 rows 42 and 48. No sequence has more
 // than one row (or the rows happen to be spread unevenly) when there are no more rows than sequences: one kernel.
 constexpr int kKv4FewRows = 64;
 template <int kDim>

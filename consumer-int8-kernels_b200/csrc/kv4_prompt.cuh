@@ -14,9 +14,9 @@
 // What bounds it is not the tensor pipe (37 to 40 % busy) but what feeds it. Dim 256, where a tile of keys serves 128 rows
 // only: the unpacking (11 instructions and one 16-byte store for eight components), ahead of the shared memory's bandwidth.
 // Dim 128: the chain scores -> softmax -> product -> next scores of each query tile, of which two run at a time, with 37 %
-// of the cycles taken by the exponentials. Measured (32 query heads and 8 key heads of 128, 8192 new tokens): 747 us,
-// 736 TFLOP/s; 24 and 4 heads of 256, 4096 tokens behind 4096: 767 us, 807 TFLOP/s, where queries in shared memory and lanes
-// that load from eight rows at a time took 1020; 32 and 8 heads of 64, 8192 tokens: 640 us. Tried and slower: tiles of 64 keys
+// of the cycles taken by the exponentials. Measured (32 query heads and 8 key heads of 128, 8192 new tokens): 748 us,
+// 735 TFLOP/s; 24 and 4 heads of 256, 4096 tokens behind 4096: 762 us, 812 TFLOP/s, where queries in shared memory and lanes
+// that load from eight rows at a time took 1020; 32 and 8 heads of 64, 8192 tokens: 636 us. Tried and slower: tiles of 64 keys
 // with two score buffers for dim 128 (792), the tiles of keys dealt to two softmax warpgroups in turn (831; dim 256 880
 // against 876 then), four unpacking warpgroups for dim 256 (917 against 876), more registers for the softmax (782 to 821).
 #pragma once

@@ -6,8 +6,9 @@
 // stands for scale * (c - zero). Codes and pairs of a block are contiguous, so a run of tokens inside a page
 // is two contiguous pieces and any page starts on a 16-byte boundary.
 //
-// A head of dim components is handled by dim / 8 neighbouring lanes of a warp, eight components (one
-// 16-byte load) each, so a warp holds 4, 2 or 1 heads (dim 64, 128, 256) and all reductions are shuffles.
+// A head of dim components is handled by dim / 8 neighbouring lanes of a warp, eight components each (one
+// 16-byte load, or two of 8 bytes where the lane holds both runs that a rotation pairs), so a warp holds 4, 2
+// or 1 heads (dim 64, 128, 256) and all reductions are shuffles.
 #pragma once
 #include <cuda_bf16.h>
 #include <cstdint>
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256, 4) kv4_rows_kernel(const Kv4RowParams p) 
   uint8_t* slot_page = nullptr;
   int slot_row = 0;
   const int page = 1 << p.page_shift;
-  const unsigned block_bytes = page * (kDim / 2 + 4);    // at most 32 KB
+  const unsigned block_bytes = page * (kDim / 2 + 4);    // at most 33792
   if (kAppend && kind > 0) {
     const int64_t slot = p.slots[token];
     if (slot >= p.capacity && lane == 0) atomicOr(&g_ci8_status, kStatusBadIndex);

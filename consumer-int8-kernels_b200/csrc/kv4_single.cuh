@@ -1,8 +1,8 @@
 // Attention of few query rows per sequence (generated tokens) over the 4-bit key/value cache: bound by reading the
 // cache, dim / 2 + 4 bytes per token and side, and as much by the instructions that unpack it: 530 for a warp's 32 keys of 128
 // components (16 + 16 of them matrix products), with the schedulers issuing in 56 % of the cycles and the logic pipe
-// busy in 50 %. Measured: 64 sequences of up to 8192 keys, 32 query heads and 8 key heads of 128, 75 us (4.0 TB/s); 4 of 65536,
-// 24 and 4 heads of 256, 78 us (3.6 TB/s); one of 1000 keys 11.5 us, most of it a chain of dependent loads and joins. The same
+// busy in 50 %. Measured: 64 sequences of up to 8192 keys, 32 query heads and 8 key heads of 128, 76 us (3.9 TB/s); 4 of 65536,
+// 24 and 4 heads of 256, 77 us (3.6 TB/s); one of 1000 keys 12 us, most of it a chain of dependent loads and joins. The same
 // loads without the arithmetic reach 5.6 TB/s.
 //
 // Work is cut into tiles of 64 tokens (32 for dim 256) of one (sequence, key head, block of query rows) and the tiles of all of
@@ -18,8 +18,9 @@
 // (two cycles a mask-and-or), so each product takes the form that needs the fewest:
 //   S^T  INT8 (m16n8k32): two masks give the eight codes of a word. The queries become 16-bit fixed point, two INT8
 //        digits relative to the row's largest component, two exact integer products; a query component is off by at
-//        most 2^-17 of the largest, a score of BF16 queries whose components lie within a factor 128 by less than the
-//        queries' own rounding. The sums, less zero * sum of q, stay exact until the key's scale is applied in FP32.
+//        most 1 / 65278 of the largest (half a step, 2^-16), which for BF16 components within a factor 128 of it is no more
+//        than their own rounding (2^-9 of a component at least). The sums, less zero * sum of q, are exact integers, rounded
+//        once to FP32 (they may have 28 bits) and then multiplied by the row's unit and the key's scale.
 //   O^T  FP16 (m16n8k16): a mask-and-or gives 1024 + code or 1024 + 16 * code for two tokens, one packed FMA the exact
 //        small integer code - zero (not zero points taken out of the sum afterwards: a sum over the whole history
 //        would cancel). The weights carry the values' scales, relative to the largest scale that the row has seen so far, which
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(Kv4SingleConfig<kDim, kQ>::kWarps * 32, 1) kv4
   }
   const long long all_tiles = __shfl_sync(0xffffffffu, sums, kWarps - 1);
   if (all_tiles == 0) return;
-  if (all_tiles >> 31) {                                 // only overlapping sequences can come to that: refused
+  if (all_tiles >> 31) {                                 // 10^11 keys, many minutes of work, or overlapping sequences: refused
     if (thread == 0) atomicOr(&g_ci8_status, kStatusBadIndex);
     return;
   }

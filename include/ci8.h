@@ -220,7 +220,10 @@ int ci8_peer_rendezvous(void* const* signals, void* state, int world, int rank, 
  * Cache: UINT8 [pages, 2 (0 keys, 1 values), kv_heads, page * (dim / 2 + 4)], 16-byte aligned; page = 16, 32, 64,
  * 128 or 256 tokens, dim = 64, 128 or 256. The block of (page, side, head) holds `page` rows of dim / 2 bytes
  * (byte j: component 2j in the low and 2j + 1 in the high four bits), then `page` pairs of BF16 numbers (scale,
- * zero point); a code c stands for scale * (c - zero). Slot s of the cache is row s % page of page s / page.
+ * zero point); a code c stands for scale * (c - zero). Slot s of the cache is row s % page of page s / page. A cache
+ * that something other than ci8_kv4_append fills has to keep to what that writes: the zero point a whole number from 0 to
+ * 15, the scale finite and above 0 (both 0 in rows of a cleared cache, which stand for zeros). Other pairs lead to no
+ * access outside a buffer, but each operator rounds them in its own way.
  *
  * Heads tensors are BF16 [tokens, heads, dim] with a token stride given in elements (a multiple of 8), 16-byte
  * aligned, so that slices of one projection's output can be passed. Head counts up to 1024.
@@ -272,7 +275,13 @@ long long ci8_kv4_workspace_bytes(void);
  * 0 < scale < 2.3e38 (times log2 e it has to be an FP32 number), width * page at most 2^30. Rows that see nothing are zeros;
  * rows of no sequence are left as they were. Lengths are cut to the table's width; tokens of a page number outside the cache are
  * not seen (status bit 3), and entries behind a sequence's last page are not read. All lengths are read on the device, so a
- * captured call follows their values. */
+ * captured call follows their values.
+ * Range: a row whose query holds a NaN or an infinity is NaN where it sees a key, and so is one whose scores, or whose products
+ * q k before the scale, leave FP32's range; neither reaches other rows. Values up to the infinities that ci8_kv4_append
+ * holds as 8.5e37 are fine. Weights times value scales are rounded to BF16 for sequences of more than 64 query rows (tokens
+ * times query heads per key head) in calls with more rows than sequences, and otherwise to FP16, relative to the largest value
+ * scale that the row sees: there what is below 2^-31 of that is lost. out and workspace must not overlap any other argument. A
+ * call of 2^31 tiles of 64 keys (32 for dim 256) and eight or sixteen query rows is not carried out (status bit 3). */
 int ci8_kv4_attention(const void* q, long long q_stride, const void* cache, const int32_t* block_table, const int32_t* q_starts,
                       const int32_t* kv_lens, void* workspace, void* out, int tokens, int batch, int width, int pages, int page,
                       int q_heads, int kv_heads, int dim, float scale, ci8_stream_t stream);
