@@ -44,4 +44,11 @@ __device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4AttendParams& p, in
   return s;
 }
 
+// 2^x within a relative error of 2^-22.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 }  // namespace ci8

@@ -125,12 +125,6 @@ __device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&v
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float kv4_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -394,7 +388,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float next = fmaxf(m[r], top[r]);
-            keep[r] = next == -INFINITY ? 1.f : kv4_exp2(m[r] - next);
+            keep[r] = next == -INFINITY ? 1.f : fast_exp2(m[r] - next);
             m[r] = next;
             sum2[r].x *= keep[r];
             sum2[r].y *= keep[r];
@@ -435,7 +429,7 @@ __global__ void __launch_bounds__(512, 1) kv4_prompt_kernel(const Kv4PromptParam
             for (int r = 0; r < 4; ++r) {
               const uint32_t* at = &s[h][r / 2][4 * i + 2 * (r & 1)];
               float2 x = __fadd2_rn(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), base2[r]);
-              x = make_float2(kv4_exp2(x.x), kv4_exp2(x.y));
+              x = make_float2(fast_exp2(x.x), fast_exp2(x.y));
               sum2[r] = __fadd2_rn(sum2[r], x);
               x = __fmul2_rn(x, v);
               packed[r / 2][2 * i + (r & 1)] = pack2(x.x, x.y);
@@ -765,7 +759,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(const Kv4PromptPar
       const float sum = __ldcg(piece(s) + 128 + row % 128), top = __ldcg(piece(s) + row % 128);
       float4 y = __ldcg(reinterpret_cast<const float4*>(piece(s) + 256 + row % 128 * kDim + column));
       // a part that saw no key has sum 0 and left its output unwritten (a NaN score makes its sum NaN, which is kept)
-      const float weight = sum == 0.f ? 0.f : kv4_exp2(top - most);
+      const float weight = sum == 0.f ? 0.f : fast_exp2(top - most);
       if (sum == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
       all += weight * sum;
       x.x += weight * y.x; x.y += weight * y.y; x.z += weight * y.z; x.w += weight * y.w;

@@ -91,11 +91,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float fast_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // Four-bit codes of two tokens, at bits 0..3 and 16..19 of w (i = 0) or at bits 4..7 and 20..23 (i = 1), less the tokens'
 // zero points, as FP16: the mask-and-or gives 1024 + code (1024 + 16 * code), and what is subtracted is 1024 + zero
 // (64 + zero).
